@@ -33,6 +33,8 @@ extern "C" {
 #define MINIKV_ABI_VERSION 1
 
 enum { MINIKV_F32 = 0, MINIKV_F16 = 1, MINIKV_BF16 = 2 };
+/* pool code of a 4-bit KV pool, beside the dtype codes (minikv_block_bounds_update) */
+enum { MINIKV_INT4 = 3 };
 /* FP8 KV pool byte formats (OCP FP8). */
 enum { MINIKV_FP8_E4M3 = 0, MINIKV_FP8_E5M2 = 1 };
 enum { MINIKV_OK = 0, MINIKV_EINVAL = 1, MINIKV_ECUDA = 2, MINIKV_EUNSUPPORTED = 3 };
@@ -290,6 +292,122 @@ int minikv_paged_prefill(const void* q, const void* key_cache, const void* value
                          int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
                          int64_t head_dim, int64_t num_blocks, int64_t block_size,
                          int64_t table_width, int64_t max_query_len, int dtype, void* stream);
+
+/* ------------------------------------------------------------ 4-bit KV pool ---
+ * No counterpart in the reference.  A pool is [num_blocks, kv_heads,
+ * minikv_int4_page_bytes(block_size, head_dim)] bytes.  The page of one kv head
+ * is block_size rows of head_dim/2 bytes (element 2i in the low half of byte
+ * i), then block_size pairs of fp16 (step, base), padded to 16 bytes.  An
+ * element reads as base + step * code; a stored step below 2^-24 reads as
+ * 2^-24.  A row (one token, one kv head, K or V) is quantised by itself:
+ *   base = fp16(min), step = fp16(max(2^-24, (max - min) / 15)),
+ *   code = round((x - base) / step) clamped to 0..15 (nearest even),
+ * with NaN counted as 0 and magnitudes saturated at 65504.  head_dim in {32,
+ * 64, 96, 128, 192, 256}; any block_size.  Returns -1 for other shapes. */
+int64_t minikv_int4_page_bytes(int64_t block_size, int64_t head_dim);
+
+/* Quantising writes from fp32/fp16/bf16 rows, with the destinations of
+ * minikv_kv_scatter_slots and minikv_kv_append_batch (rows outside are
+ * skipped); a source row's heads are contiguous, its alignment and token
+ * stride are free. */
+int minikv_kv_scatter_slots_int4(void* key_cache, void* value_cache, const int64_t* slot_mapping, const void* key,
+                                 const void* value, int64_t tokens, int64_t num_blocks, int64_t block_size,
+                                 int64_t kv_heads, int64_t head_dim, int64_t key_token_stride,
+                                 int64_t value_token_stride, int dtype, void* stream);
+int minikv_kv_append_batch_int4(void* key_cache, void* value_cache, const int64_t* block_tables,
+                                const int64_t* token_offsets, const void* key, const void* value, int64_t batch,
+                                int64_t table_width, int64_t num_blocks, int64_t block_size, int64_t kv_heads,
+                                int64_t head_dim, int64_t key_token_stride, int64_t value_token_stride, int dtype,
+                                void* stream);
+
+/* The values of slots, as contiguous [tokens, kv_heads, head_dim] rows of
+ * `dtype` (the fp32 value rounded once); zeros for a slot outside the pool. */
+int minikv_kv_gather_slots_int4(const void* key_cache, const void* value_cache, const int64_t* slot_mapping, void* key,
+                                void* value, int64_t tokens, int64_t num_blocks, int64_t block_size, int64_t kv_heads,
+                                int64_t head_dim, int dtype, void* stream);
+
+/* Decode attention over a 4-bit pool: minikv_paged_decode's contract and
+ * guards with an fp16/bf16 query and output.  `selected` (may be null): the
+ * logical blocks each kv head attends, [batch, kv_heads, max_blocks] int64, as
+ * minikv_select_blocks gives them; the first min(max_blocks, blocks of the
+ * request) entries of a row are read, an entry outside the request masks its
+ * tokens.  tickets: device memory of batch * kv_heads *
+ * ceil(q_heads / kv_heads / 8) 32-bit counters, zero before its first use; every
+ * call, of whatever shape, leaves it zero.  workspace: scratch of the size
+ * asked for, of any content.  Calls that share either must not overlap. */
+int64_t minikv_paged_decode_int4_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                 int64_t num_blocks, int64_t block_size, int64_t table_width,
+                                                 int dtype);
+int minikv_paged_decode_int4(const void* query, const void* key_cache, const void* value_cache,
+                             const int64_t* block_tables, const int64_t* context_lens, const int64_t* selected,
+                             void* out, void* tickets, void* workspace, int64_t workspace_bytes, int64_t batch,
+                             int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks,
+                             int64_t block_size, int64_t table_width, int64_t max_blocks, int dtype, void* stream);
+
+/* Ragged causal prefill over a 4-bit pool: minikv_paged_prefill's contract with
+ * an fp16/bf16 query and output and up to 64 query heads a kv head; no
+ * workspace.  Tokens of no request, or past their context, get zero rows. */
+int minikv_paged_prefill_int4(const void* q, const void* key_cache, const void* value_cache,
+                              const int64_t* cu_seqlens_q, const int64_t* query_starts, const int64_t* block_tables,
+                              const int64_t* context_lens, void* out, int64_t tokens, int64_t requests,
+                              int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks,
+                              int64_t block_size, int64_t table_width, int64_t max_query_len, int dtype, void* stream);
+
+/* ---------------------------------------------------------- block selection ---
+ * No counterpart in the reference.  Attention that reads, for each request and
+ * kv head, only the blocks (pages) whose keys can score highest.
+ *
+ * Bounds: [num_blocks, kv_heads, 2 * head_dim + 16] bytes, one record per block
+ * and kv head: head_dim int8 codes of the keys' elementwise maximum, head_dim of
+ * their minimum, one fp32 scale = top / 127 (top: the largest magnitude of the
+ * 2 * head_dim bounds), 12 zero bytes.  Codes are ceil(127 max / top) and
+ * floor(127 min / top); a bound reads as code * scale.  A top below 2^-100
+ * gives a zero record.  NaN keys count as 0, infinite ones as the largest fp32.
+ *
+ * Update the records of the blocks that hold rows [query_starts[r],
+ * context_lens[r]) of each request, from all of the blocks' rows below
+ * context_lens[r].  key_cache: [num_blocks, block_size, kv_heads, head_dim] of
+ * the dtype `pool`, or a 4-bit pool (pool = MINIKV_INT4).  max_query_len bounds
+ * context_lens[r] - query_starts[r]; blocks past the bound are not updated.
+ * Requests and pages out of range are skipped. */
+int minikv_block_bounds_update(void* bounds, const void* key_cache, const int64_t* block_tables,
+                               const int64_t* query_starts, const int64_t* context_lens, int64_t requests,
+                               int64_t table_width, int64_t num_blocks, int64_t block_size, int64_t kv_heads,
+                               int64_t head_dim, int64_t max_query_len, int pool, void* stream);
+
+/* Values of the bounds of listed blocks: lower and upper [count, kv_heads,
+ * head_dim] fp32; zeros for a block outside the pool. */
+int minikv_block_bounds_read(const void* bounds, const int64_t* block_ids, int64_t count, float* lower, float* upper,
+                             int64_t num_blocks, int64_t kv_heads, int64_t head_dim, void* stream);
+
+/* The max_blocks blocks of highest score of each request and kv head, in
+ * ascending order, -1 behind the last: selected [batch, kv_heads, max_blocks].
+ * score = scale * (sum_d maxcode_d qp_d + mincode_d qn_d), with qp and qn the
+ * 8-bit codes, over their common largest magnitude, of the kv head's summed
+ * positive and negative query parts; the sum is a whole number, so the
+ * selection does not depend on the order of evaluation.  Ties go to the lowest
+ * block.  The first sink_blocks and the last recent_blocks of a request are
+ * taken whatever their scores (sink_blocks + recent_blocks <= max_blocks);
+ * blocks without a page of the pool are not; an out-of-range length selects
+ * nothing.  The query may be fp32/fp16/bf16.  workspace: scratch of any content. */
+int64_t minikv_select_blocks_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t table_width);
+int minikv_select_blocks(const void* query, const void* bounds, const int64_t* block_tables,
+                         const int64_t* context_lens, int64_t* selected, void* workspace, int64_t workspace_bytes,
+                         int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks,
+                         int64_t block_size, int64_t table_width, int64_t max_blocks, int64_t sink_blocks,
+                         int64_t recent_blocks, int dtype, void* stream);
+
+/* Decode attention over the selected blocks of a 16-bit pool (fp16/bf16,
+ * head_dim in {32, 64, 96, 128, 192, 256}); `selected`, tickets and workspace
+ * as for minikv_paged_decode_int4. */
+int64_t minikv_paged_decode_selected_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                     int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                                                     int64_t table_width, int dtype);
+int minikv_paged_decode_selected(const void* query, const void* key_cache, const void* value_cache,
+                                 const int64_t* block_tables, const int64_t* context_lens, const int64_t* selected,
+                                 void* out, void* tickets, void* workspace, int64_t workspace_bytes, int64_t batch,
+                                 int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks,
+                                 int64_t block_size, int64_t table_width, int64_t max_blocks, int dtype, void* stream);
 
 /* -------------------------------------------------------------- metadata ---
  * Device-side construction of the ragged prefill batch metadata of

@@ -49,6 +49,19 @@ SIGNATURES = {
     "minikv_copy_blocks": (_int, [_p, _p, _p] + [_i64] * 4 + [_int, _p]),
     "minikv_paged_prefill_workspace_bytes": (_i64, [_i64] * 9 + [_int]),
     "minikv_paged_prefill": (_int, [_p] * 8 + [_p, _i64] + [_i64] * 9 + [_int, _p]),
+    "minikv_int4_page_bytes": (_i64, [_i64, _i64]),
+    "minikv_kv_scatter_slots_int4": (_int, [_p] * 5 + [_i64] * 7 + [_int, _p]),
+    "minikv_kv_append_batch_int4": (_int, [_p] * 6 + [_i64] * 8 + [_int, _p]),
+    "minikv_kv_gather_slots_int4": (_int, [_p] * 5 + [_i64] * 5 + [_int, _p]),
+    "minikv_paged_decode_int4_workspace_bytes": (_i64, [_i64] * 7 + [_int]),
+    "minikv_paged_decode_int4": (_int, [_p] * 9 + [_i64] + [_i64] * 8 + [_int, _p]),
+    "minikv_paged_prefill_int4": (_int, [_p] * 8 + [_i64] * 9 + [_int, _p]),
+    "minikv_block_bounds_update": (_int, [_p] * 5 + [_i64] * 7 + [_int, _p]),
+    "minikv_block_bounds_read": (_int, [_p, _p, _i64, _p, _p] + [_i64] * 3 + [_p]),
+    "minikv_select_blocks_workspace_bytes": (_i64, [_i64] * 3),
+    "minikv_select_blocks": (_int, [_p] * 6 + [_i64] + [_i64] * 10 + [_int, _p]),
+    "minikv_paged_decode_selected_workspace_bytes": (_i64, [_i64] * 7 + [_int]),
+    "minikv_paged_decode_selected": (_int, [_p] * 9 + [_i64] + [_i64] * 8 + [_int, _p]),
     "minikv_build_prefill_metadata": (_int, [_p] * 5 + [_i64] * 4 + [_p] * 7 + [_p]),
     "minikv_build_decode_tables": (_int, [_p] * 6 + [_i64, _i64] + [_p] * 3 + [_p]),
     "minikv_rms_norm": (_int, [_p] * 5 + [_i64, _i64, ctypes.c_double, _int, _p]),

@@ -2,8 +2,9 @@
 
     python -m myvllm_mini_engine_b200.build [--verbose]
 
-One translation unit (csrc/abi.cu includes the kernel files), compiled with
-``-gencode arch=compute_100a,code=sm_100a -O3 -lineinfo``.  The CUDA runtime
+The translation units (``UNITS``; each includes its kernel files) are compiled
+side by side with ``-gencode arch=compute_100a,code=sm_100a -O3 -lineinfo`` and
+linked.  The CUDA runtime
 is linked statically, so the library only needs the NVIDIA driver at run time.
 
 The SHA-256 of the sources (``source_hash()``) is compiled into the library
@@ -20,6 +21,7 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -27,7 +29,8 @@ ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 OUTPUT = PACKAGE / "libminikv.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
+FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
+UNITS = ("abi", "pages_abi", "source_hash")
 
 
 def sources():
@@ -71,15 +74,26 @@ def up_to_date() -> bool:
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and up_to_date():
         return OUTPUT
-    tmp = OUTPUT.with_suffix(".so.tmp")
-    cmd = [nvcc_path(), *ARCH, *FLAGS, f'-DMINIKV_SOURCE_HASH="{source_hash()}"', "-o", str(tmp),
-           str(CSRC / "abi.cu")]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), flush=True)
-    result = subprocess.run(cmd, capture_output=not verbose, text=True)
-    if result.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({result.returncode}):\n{result.stderr if not verbose else ''}")
+    with tempfile.TemporaryDirectory() as scratch:
+        objects, running = [], []
+        for unit in UNITS:
+            objects.append(str(Path(scratch) / f"{unit}.o"))
+            cmd = [nvcc_path(), *ARCH, *FLAGS, f'-DMINIKV_SOURCE_HASH="{source_hash()}"', "-c", "-o", objects[-1],
+                   str(CSRC / f"{unit}.cu")]
+            if verbose:
+                cmd.insert(1, "-Xptxas=-v")
+                print(" ".join(cmd), flush=True)
+            running.append(subprocess.Popen(cmd, stderr=None if verbose else subprocess.PIPE, text=True))
+        tmp = OUTPUT.with_suffix(".so.tmp")
+        errors = [process.communicate()[1] for process in running]
+        link = [nvcc_path(), *ARCH, "-shared", "-o", str(tmp), *objects]
+        if all(process.returncode == 0 for process in running):
+            result = subprocess.run(link, stderr=None if verbose else subprocess.PIPE, text=True)
+            running.append(result)
+            errors.append(result.stderr)
+        for process, error in zip(running, errors):
+            if process.returncode != 0:
+                raise RuntimeError(f"nvcc failed ({process.returncode}):\n{error or ''}")
     os.replace(tmp, OUTPUT)
     return OUTPUT
 

@@ -90,15 +90,12 @@ extern "C" {
 
 int minikv_abi_version(void) { return MINIKV_ABI_VERSION; }
 
-#ifndef MINIKV_SOURCE_HASH
-#define MINIKV_SOURCE_HASH "unknown"
-#endif
-// The marker prefix lets the build recipe read the hash from the file without loading it.
-static const char kSourceHash[] = "minikv-source-hash:" MINIKV_SOURCE_HASH;
-
-const char* minikv_source_hash(void) { return kSourceHash + sizeof("minikv-source-hash:") - 1; }
-
 const char* minikv_last_error(void) { return g_last_error.c_str(); }
+
+// The message of a failed call in another translation unit of the library.
+__attribute__((visibility("hidden"))) int minikv_set_error(int code, const char* message) {
+    return fail(code, message);
+}
 
 int minikv_device_status(unsigned int* status, int clear, void* stream) {
     MINIKV_REQUIRE(status != nullptr, MINIKV_EINVAL, "status pointer is null");

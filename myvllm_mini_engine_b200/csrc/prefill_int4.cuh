@@ -1,0 +1,392 @@
+// Ragged causal prefill over a 4-bit pool.
+//
+// Packed query token i of request r sits at position start + i and attends the
+// keys [0, start + i] of r's pages (history and current chunk, already written).
+// A CTA takes 64 rows, (token, query head) pairs of one request and kv head, 16
+// a warp, and goes over the keys BN at a time with a running maximum and sum:
+//   S = Q K^T,  s = (step (q . c) + base sum(q)) / sqrt(D),  P = 2^(s - max)
+//   O += (P step') C'^T,  z += P base',  out = (O + z) / sum P
+// As in decode_pages.cuh the codes are the operands, nibbles masked out of the
+// staged words (fp16 subnormals c 2^-24, c 2^-20; Q of the latter is scaled by
+// 1/16 beforehand, so one accumulator serves both).  P step' is scaled by the
+// power of two above the largest step met so far (raising it rescales O), so
+// that it stays in fp16's normal range whatever the steps are, and rounded to
+// fp16 once: 2^-12 next to the output's own 2^-12 (fp16) or 2^-9 (bf16).
+//
+// Bound by the tensor pipe and by issue: a warp makes its operands from the
+// codes itself.  mma.sync rather than tcgen05: a tcgen05 operand has to lie in
+// shared memory as 16-bit values, four times the codes' bytes written there and
+// read back per tile, while the masked registers feed mma.sync as they are and
+// the P operand never leaves them.
+#pragma once
+
+#include "decode_pages.cuh"
+
+namespace minikv {
+
+struct PrefillInt4Params {
+    const void* q;
+    const unsigned char* kc;
+    const unsigned char* vc;
+    const int64_t* cu;
+    const int64_t* starts;
+    const int64_t* tables;
+    const int64_t* lens;
+    void* out;
+    int64_t tokens, width, num_blocks, page_bytes;
+    int requests, q_heads, kv_heads, group, block_size, tile_tokens;  // tile_tokens: 64 / group
+    uint64_t bs_magic;
+    float scale_log2;
+};
+
+constexpr int kPrefillWarps = 4;
+constexpr int kPrefillThreads = kPrefillWarps * 32;
+constexpr int kPrefillRows = kPrefillWarps * 16;
+constexpr int kPrefillStages = 3;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 2 : 1) prefill_int4_kernel(const PrefillInt4Params p) {
+    constexpr int BN = D <= 128 ? 64 : 32;  // keys a tile: the accumulators of S take BN / 2 registers
+    constexpr int RB = D / 2, CPR = RB / 16, NW = D / 32, NT = BN / 8;
+    constexpr int STAGE = BN * (2 * RB + 8);  // K codes, V codes, K pairs, V pairs
+    __shared__ __align__(128) unsigned char ring[kPrefillStages * STAGE];
+    __shared__ int64_t row_at[2][BN];     // byte of a key's codes in the pool, or -1
+    __shared__ int64_t pair_at[2][BN];
+    __shared__ uint32_t valid_s[kPrefillStages][2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
+    const int kvh = blockIdx.x, r = blockIdx.z;
+    griddep_wait();
+    griddep_launch_dependents();
+    const int64_t cu0 = p.cu[r], cu1 = p.cu[r + 1], start = p.starts[r], len = p.lens[r];
+    const int64_t* table = p.tables + (int64_t)r * p.width;
+    T* out = static_cast<T*>(p.out);
+    // ---- packed tokens of no request get zeros
+    if (r == 0 || r == p.requests - 1) {
+        const int64_t heads = p.group * D;
+        auto zero = [&](int64_t a, int64_t b) {
+            a = a < 0 ? 0 : a;
+            b = b > p.tokens ? p.tokens : b;
+            for (int64_t x = (int64_t)blockIdx.y * kPrefillThreads + tid; x < (b - a) * heads;
+                 x += (int64_t)gridDim.y * kPrefillThreads)
+                out[((a + x / heads) * p.q_heads + (int64_t)kvh * p.group) * D + x % heads] = Elem<T>::from_float(0.f);
+        };
+        if (r == 0) zero(0, cu0);
+        if (r == p.requests - 1) zero(cu1, p.tokens);
+    }
+    if (cu0 < 0 || cu1 > p.tokens || cu0 >= cu1) return;
+    const int64_t count = cu1 - cu0;
+    const int64_t tiles = (count + p.tile_tokens - 1) / p.tile_tokens;
+    const int64_t reach = min(len, p.width * (int64_t)p.block_size);  // keys that exist
+
+    // the latest tiles, which see the most keys, come first
+    for (int64_t qt = tiles - 1 - blockIdx.y; qt >= 0; qt -= gridDim.y) {
+        const int64_t i0 = qt * p.tile_tokens;
+        const int here = (int)min((int64_t)p.tile_tokens, count - i0);  // tokens of this tile
+        // ---- rows of this lane: warp * 16 + g and + 8
+        int64_t row_out[2];
+        int last[2];  // last visible key of the row, -1: none
+        uint32_t qa[2 * NW][4];
+        float qsum[2], qscale[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int row = warp * 16 + g + 8 * x;
+            const int tok = row / p.group, hd = row - tok * p.group;
+            const bool in = tok < here;
+            row_out[x] = in ? ((cu0 + i0 + tok) * p.q_heads + (int64_t)kvh * p.group + hd) * D : -1;
+            const int64_t pos = start + i0 + tok;
+            last[x] = in && pos >= 0 && pos < reach ? (int)pos : -1;
+            float f[8 * NW];
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8 * NW; i += 8) {
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (in) v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + row_out[x] + q4 * (D / 4) + i);
+                Elem<T>::load(v, f + i);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[i + e]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // scaled by a power of two into [1, 2), as in the decode
+            const int e2 = (top > 0.f && top < INFINITY)
+                               ? min(120, max(-120, (int)((__float_as_uint(top) >> 23) & 255) - 127)) : 0;
+            const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                float y[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    y[i] = __half2float(__float2half_rn(f[8 * w + i] * down));
+                    // the operand of a high nibble, 16 times larger as a subnormal
+                    if (i & 1) {
+                        const float small = __half2float(__float2half_rn(y[i] * 0.0625f));
+                        y[i] = small;
+                        sum += small * 16.f;
+                    } else {
+                        sum += y[i];
+                    }
+                }
+                qa[2 * w][x] = Elem<__half>::pack(y[0], y[4]);
+                qa[2 * w][2 + x] = Elem<__half>::pack(y[2], y[6]);
+                qa[2 * w + 1][x] = Elem<__half>::pack(y[1], y[5]);
+                qa[2 * w + 1][2 + x] = Elem<__half>::pack(y[3], y[7]);
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            qsum[x] = sum;
+            qscale[x] = __uint_as_float((uint32_t)(127 + e2) << 23) * p.scale_log2;
+        }
+        // a row past the context sees nothing, whatever its neighbours see
+        const bool odd_rows = __any_sync(0xffffffffu, (row_out[0] >= 0 && last[0] < 0) || (row_out[1] >= 0 && last[1] < 0));
+        // ---- keys this tile sees, and those that all of the warp's rows see
+        const int64_t far = start + i0 + here - 1;
+        const int keys = (int)max((int64_t)0, min(reach, far + 1));
+        const int warp_near = (int)max((int64_t)0, min(reach, start + i0 + (warp * 16) / p.group + 1));
+        const int nk = (keys + BN - 1) / BN;
+
+        auto look = [&](int kt) {  // threads below BN: where the tile's keys lie
+            if (tid < BN) {
+                const int pos = kt * BN + tid;
+                int64_t at = -1, pair = -1;
+                if (pos < keys) {
+                    const int e = (int)(((uint64_t)pos * p.bs_magic) >> 42);
+                    const int64_t page = table[e];
+                    if (page >= 0 && page < p.num_blocks) {
+                        const int off = pos - e * p.block_size;
+                        const int64_t base = (page * p.kv_heads + kvh) * p.page_bytes;
+                        at = base + (int64_t)off * RB;
+                        pair = base + (int64_t)p.block_size * RB + off * 4;
+                    }
+                }
+                row_at[kt & 1][tid] = at;
+                pair_at[kt & 1][tid] = pair;
+            }
+        };
+        auto copy = [&](int kt) {
+            if (kt < nk) {
+                const int s = kt % kPrefillStages;
+                const uint32_t dst = smem_addr(ring) + s * STAGE;
+#pragma unroll
+                for (int c0 = 0; c0 < BN * CPR; c0 += kPrefillThreads) {
+                    const int c = c0 + tid;
+                    if (BN * CPR % kPrefillThreads == 0 || c < BN * CPR) {
+                        const int row = c / CPR, x = c - row * CPR;
+                        const int64_t at = row_at[kt & 1][row];
+                        const int64_t from = at < 0 ? 0 : at + x * 16;
+                        const uint32_t n = at < 0 ? 0u : 16u;
+                        copy16(dst + row * RB + x * 16, p.kc + from, n);
+                        copy16(dst + (BN + row) * RB + x * 16, p.vc + from, n);
+                    }
+                }
+                if (tid < 2 * BN) {
+                    const int64_t at = pair_at[kt & 1][tid % BN];
+                    copy4(dst + 2 * BN * RB + tid * 4, (tid < BN ? p.kc : p.vc) + (at < 0 ? 0 : at), at < 0 ? 0u : 4u);
+                }
+                if (tid < BN) {
+                    const uint32_t bits = __ballot_sync(0xffffffffu, row_at[kt & 1][tid] >= 0);
+                    if (lane == 0) valid_s[s][warp] = bits;
+                }
+            }
+            copy_commit();
+        };
+        __syncthreads();  // the ring and the look-ups of the tile before are free
+        look(0);
+        __syncthreads();
+        copy(0);
+        look(1);
+        __syncthreads();
+        copy(1);
+        // (the loop's first barrier comes before look(2) is needed)
+
+        float o[NW][4][4];
+#pragma unroll
+        for (int u = 0; u < NW; ++u)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[u][n][i] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, z[2] = {0.f, 0.f};
+        int vexp = -26;  // steps so far are below 2^(vexp + 1)
+
+        for (int kt = 0; kt < nk; ++kt) {
+            copy_wait<1>();
+            look(kt + 2);     // the look-ups of tile kt, whose buffer this takes, were used by copy(kt)
+            __syncthreads();  // tile kt is whole; every warp is done with tile kt - 1
+            copy(kt + 2);
+            const unsigned char* st = ring + (kt % kPrefillStages) * STAGE;
+            const uint64_t valid = valid_s[kt % kPrefillStages][0] |
+                                   (BN > 32 ? (uint64_t)valid_s[kt % kPrefillStages][1] << 32 : 0ull);
+            const __half2* kp = reinterpret_cast<const __half2*>(st + 2 * BN * RB);
+            const __half2* vp = kp + BN;
+            // ---- S: column c of key group j is its key c / 2 + 4 (c % 2)
+            float s[NT][4];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const unsigned char* src = st + (8 * j + (g >> 1) + 4 * (g & 1)) * RB + q4 * (RB / 4);
+                uint32_t w[NW];
+                if constexpr (NW % 4 == 0) {
+#pragma unroll
+                    for (int i = 0; i < NW / 4; ++i) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(src + 16 * i);
+                        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NW; ++i) w[i] = *reinterpret_cast<const uint32_t*>(src + 4 * i);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+                    mma16816<__half>(s[j], qa[2 * i], w[i] & kNibbleMask, (w[i] >> 8) & kNibbleMask);
+                    mma16816<__half>(s[j], qa[2 * i + 1], w[i] & (kNibbleMask << 4),
+                                     (w[i] >> 8) & (kNibbleMask << 4));
+                }
+            }
+            const bool edge = odd_rows || (kt + 1) * BN > warp_near || valid != (BN == 64 ? ~0ull : 0xffffffffull);
+            float vmax = 0.f;
+            float mx[2] = {-INFINITY, -INFINITY};
+            float vs[NT][2], vb[NT][2];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const int key = 8 * j + q4 + 4 * y;
+                    const float2 a = __half22float2(kp[key]), b = __half22float2(vp[key]);
+                    const float ks = fmaxf(a.x, kInt4StepMin) * kCodeScale;
+                    vs[j][y] = fmaxf(b.x, kInt4StepMin);
+                    vb[j][y] = b.y;
+                    vmax = fmaxf(vmax, vs[j][y]);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float& e = s[j][2 * x + y];
+                        e = fmaf(e, ks, a.y * qsum[x]);
+                        if (edge && (kt * BN + key > last[x] || !((valid >> key) & 1ull))) e = -INFINITY;
+                        mx[x] = fmaxf(mx[x], e);
+                    }
+                }
+            }
+            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
+            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
+            const int ve = (int)(__float_as_uint(vmax) >> 23) - 127;
+            const int raise = max(0, ve - vexp);
+            vexp += raise;
+            const float shrink = raise > 100 ? 0.f : __uint_as_float((uint32_t)(127 - raise) << 23);
+            const float vinv = __uint_as_float((uint32_t)(127 - vexp - 1) << 23);
+            float alpha[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
+                mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
+                const float mn = fmaxf(m[x], mx[x] * qscale[x]);
+                alpha[x] = mn == -INFINITY ? 1.f : exp2_fast(m[x] - mn);
+                m[x] = mn;
+                l[x] *= alpha[x];
+                z[x] *= alpha[x];
+            }
+            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f || raise != 0)) {
+#pragma unroll
+                for (int u = 0; u < NW; ++u)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        o[u][n][0] *= alpha[0] * shrink;
+                        o[u][n][1] *= alpha[0] * shrink;
+                        o[u][n][2] *= alpha[1] * shrink;
+                        o[u][n][3] *= alpha[1] * shrink;
+                    }
+            }
+            // ---- P, and P step' as the A operand; O, 16 keys at a time
+            const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+            for (int j = 0; j < NT; j += 2) {
+                uint32_t a[4];
+#pragma unroll
+                for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float w[2];
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const float e = exp2_fast(fmaf(s[j + jj][2 * x + y], qscale[x], -mm[x]));
+                            l[x] += e;
+                            z[x] = fmaf(e, vb[j + jj][y], z[x]);
+                            w[y] = e * (vs[j + jj][y] * vinv);
+                        }
+                        a[2 * jj + x] = Elem<__half>::pack(w[0], w[1]);
+                    }
+                const unsigned char* v = st + (BN + 8 * j + q4) * RB + g * (RB / 8);
+                uint32_t x0[NW], x1[NW];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const unsigned char* va = v + half * 8 * RB;
+                    const unsigned char* vb2 = va + 4 * RB;
+                    uint32_t* dst = half ? x1 : x0;
+                    if constexpr (NW % 2 == 0) {
+                        uint32_t wa[NW / 2], wb[NW / 2];
+                        if constexpr (NW % 8 == 0) {
+                            const uint4 c = *reinterpret_cast<const uint4*>(va), d = *reinterpret_cast<const uint4*>(vb2);
+                            wa[0] = c.x; wa[1] = c.y; wa[2] = c.z; wa[3] = c.w;
+                            wb[0] = d.x; wb[1] = d.y; wb[2] = d.z; wb[3] = d.w;
+                        } else if constexpr (NW % 4 == 0) {
+                            const uint2 c = *reinterpret_cast<const uint2*>(va), d = *reinterpret_cast<const uint2*>(vb2);
+                            wa[0] = c.x; wa[1] = c.y;
+                            wb[0] = d.x; wb[1] = d.y;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < NW / 2; ++i) {
+                                wa[i] = *reinterpret_cast<const uint32_t*>(va + 4 * i);
+                                wb[i] = *reinterpret_cast<const uint32_t*>(vb2 + 4 * i);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < NW / 2; ++i) {
+                            dst[2 * i] = permute_bytes(wa[i], wb[i], 0x5410u);
+                            dst[2 * i + 1] = permute_bytes(wa[i], wb[i], 0x7632u);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NW; ++i)
+                            dst[i] = *reinterpret_cast<const uint16_t*>(va + 2 * i) |
+                                     ((uint32_t) * reinterpret_cast<const uint16_t*>(vb2 + 2 * i) << 16);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < NW; ++u) {
+                    mma16816<__half>(o[u][0], a, x0[u] & kNibbleMask, x1[u] & kNibbleMask);
+                    mma16816<__half>(o[u][1], a, x0[u] & (kNibbleMask << 4), x1[u] & (kNibbleMask << 4));
+                    mma16816<__half>(o[u][2], a, (x0[u] >> 8) & kNibbleMask, (x1[u] >> 8) & kNibbleMask);
+                    mma16816<__half>(o[u][3], a, (x0[u] >> 8) & (kNibbleMask << 4),
+                                     (x1[u] >> 8) & (kNibbleMask << 4));
+                }
+            }
+        }
+        copy_wait<0>();
+        // ---- output: lane q4 holds dims [c D/8, (c + 1) D/8) for c = 2 q4 and 2 q4 + 1
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            float L = l[x], Z = z[x];
+            L += __shfl_xor_sync(0xffffffffu, L, 1);
+            L += __shfl_xor_sync(0xffffffffu, L, 2);
+            Z += __shfl_xor_sync(0xffffffffu, Z, 1);
+            Z += __shfl_xor_sync(0xffffffffu, Z, 2);
+            if (row_out[x] < 0) continue;  // no shuffle of this row follows
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            // codes 2^-24, steps 2^-(vexp + 1): the exponent lies in [-1, 40]
+            const float up = __uint_as_float((uint32_t)(127 + vexp + 1 + 24) << 23);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                T* dst = out + row_out[x] + (2 * q4 + y) * (D / 8);
+#pragma unroll
+                for (int u = 0; u < NW; ++u) {
+                    const int i = 2 * x + y;
+                    const float f0 = fmaf(o[u][0][i], up, Z) * inv, f1 = fmaf(o[u][1][i], up * 0.0625f, Z) * inv;
+                    const float f2 = fmaf(o[u][2][i], up, Z) * inv, f3 = fmaf(o[u][3][i], up * 0.0625f, Z) * inv;
+                    *reinterpret_cast<uint2*>(dst + 4 * u) = make_uint2(Elem<T>::pack(f0, f1), Elem<T>::pack(f2, f3));
+                }
+            }
+        }
+    }
+}
+
+}  // namespace minikv

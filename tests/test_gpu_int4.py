@@ -1,0 +1,391 @@
+"""4-bit KV pool on the GPU against the CPU oracle (oracle/int4_kv.py, 64 bits).
+
+Writes match the oracle byte for byte.  Attention: with V values in a range of
+``spread`` an output is off by at most
+  half a step of its type (eps / 2 of its value), plus
+  spread * (2^-12 P' rounded to fp16 once, as bf16 outputs and the prefill have it; 2^-22 in two
+  terms) plus spread * 2 ln 2 * ds for scores off by ds (log2), where an fp32 dot product of D
+  terms is off by at most (D + 8) 2^-23 of the sum of its terms' magnitudes.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from myvllm_mini_engine_b200 import _lib
+from myvllm_mini_engine_b200.kernels import (int4_page_bytes, paged_attention_int4, paged_prefill_attention_int4,
+                                             read_kv_cache_slots_int4, write_kv_cache_batch_int4,
+                                             write_kv_cache_slots_int4)
+from oracle import int4_kv
+
+pytestmark = pytest.mark.gpu
+
+
+def randn(gen, *shape):
+    return torch.from_numpy(gen.standard_normal(shape, dtype=np.float32))
+
+
+def make_pool(gen, blocks, block_size, heads, dim, scale=1.0):
+    """A uint8 numpy pool of quantised normal rows with channel offsets."""
+    pool = np.zeros((blocks, heads, int4_kv.page_bytes(block_size, dim)), dtype=np.uint8)
+    rows = (randn(gen, blocks * block_size, heads, dim) + randn(gen, heads, dim)) * scale
+    int4_kv.scatter(pool, block_size, torch.arange(blocks * block_size), rows)
+    return pool
+
+
+def tables_for(gen, lens, block_size, spare=3):
+    width = max(1, -(-max(lens) // block_size))
+    blocks = len(lens) * width + spare
+    table = torch.from_numpy(gen.permutation(blocks)[:len(lens) * width].astype(np.int64)).view(len(lens), width)
+    return table, blocks
+
+
+def assert_near(actual, expected, query, keys, vals, dtype, one_term):
+    """The bound of the module's docstring, element by element, and half a step of the type over the whole."""
+    finite_k, finite_v = keys[torch.isfinite(keys)], vals[torch.isfinite(vals)]
+    spread = float(finite_v.max() - finite_v.min())
+    dim = query.shape[-1]
+    terms = float(query.double().abs().sum(-1).max()) * float(finite_k.abs().max()) * 2  # codes and base apart
+    ds = (dim + 8) * 2.0 ** -23 * terms * math.log2(math.e) / math.sqrt(dim)
+    inner = spread * ((2.0 ** -12 if one_term else 2.0 ** -22) + 2 * math.log(2) * ds)
+    half = torch.finfo(dtype).eps / 2
+    err = (actual.double().cpu() - expected).abs()
+    assert bool((err <= half * expected.abs() + inner + 2.0 ** -25).all()), float(err.max())
+    norm = float(expected.norm())
+    if norm:
+        assert float((actual.double().cpu() - expected).norm()) <= (half + 2.0 ** -11) * norm
+
+
+def decode(gen, dtype, lens, heads, kv_heads, dim, block_size, *, tables=None, scale=1.0, selected=None,
+           validate=True, pool_lens=None, q_scale=1.0):
+    table, blocks = tables_for(gen, pool_lens or [max(1, n) for n in lens], block_size)
+    if tables is not None:
+        table = tables(table)
+    kp, vp = make_pool(gen, blocks, block_size, kv_heads, dim, scale), make_pool(gen, blocks, block_size, kv_heads, dim, scale)
+    query = (randn(gen, len(lens), heads, dim) * q_scale).to(dtype)
+    lens = torch.tensor(lens, dtype=torch.int64)
+    keys, vals = int4_kv.values(kp, block_size, dim), int4_kv.values(vp, block_size, dim)
+    expected = int4_kv.paged_decode(query, keys, vals, table, lens, block_size, selected)
+    actual = paged_attention_int4(query.cuda(), torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(), table.cuda(),
+                                  lens.cuda(), block_size, validate=validate,
+                                  selected=None if selected is None else selected.cuda())
+    assert actual.dtype == dtype and actual.shape == query.shape
+    assert_near(actual, expected, query, keys, vals, dtype, dtype == torch.bfloat16)
+    return actual, expected
+
+
+@pytest.mark.parametrize("src", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,block_size", [(32, 5), (64, 16), (96, 16), (128, 16), (128, 1), (192, 7), (256, 24)])
+def test_writes_match_the_oracle_bytes(cuda_device, src, dim, block_size):
+    gen = np.random.default_rng(3)
+    blocks, heads = 9, 3
+    tokens = min(40, blocks * block_size)
+    sizes = torch.tensor([1e-6, 1.0, 30.0, 3e4])[torch.arange(2 * tokens) % 4]
+    data = randn(gen, 2, 2 * tokens, heads, dim) * sizes[:, None, None]
+    data[0, 0, 0, 0], data[0, 0, 1, 1] = float("nan"), float("inf")
+    data[1, 2] = 0.25                      # a constant row: step at its least, codes zero
+    data[1, 4, 0, :16] = torch.arange(16)  # codes on and between whole numbers
+    data[1, 4, 0, 16:] = torch.arange(dim - 16) % 16 + 0.5
+    data = data.to(src)
+    key, value = data[0, ::2], data[1, ::2]  # token-strided views
+    slots = torch.from_numpy(gen.permutation(blocks * block_size)[:tokens].astype(np.int64))
+    slots[1], slots[3] = -1, blocks * block_size
+    init = gen.integers(0, 256, size=(2, blocks, heads, int4_page_bytes(block_size, dim)), dtype=np.uint8)
+    want = init.copy()
+    int4_kv.scatter(want[0], block_size, slots, key)
+    int4_kv.scatter(want[1], block_size, slots, value)
+    got = torch.from_numpy(init.copy()).cuda()
+    write_kv_cache_slots_int4(got[0], got[1], slots.cuda(), key.cuda(), value.cuda(), block_size, validate=False)
+    assert np.array_equal(got.cpu().numpy(), want)
+    # misaligned sources take the element loads
+    odd = torch.zeros(data[0, ::2].numel() + 1, dtype=src, device="cuda")[1:].view(tokens, heads, dim)
+    odd.copy_(key)
+    got = torch.from_numpy(init.copy()).cuda()
+    write_kv_cache_slots_int4(got[0], got[1], slots.cuda(), odd, value.cuda(), block_size, validate=False)
+    assert np.array_equal(got.cpu().numpy(), want)
+    # the values read back
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        k, v = read_kv_cache_slots_int4(got[0], got[1], slots.cuda(), block_size, dim, dtype=dtype, validate=False)
+        for have, pool in ((k, want[0]), (v, want[1])):
+            flat = int4_kv.values(pool, block_size, dim).float().view(-1, heads, dim)
+            inside = (slots >= 0) & (slots < blocks * block_size)
+            ref = torch.where(inside[:, None, None], flat[slots.clamp(0, blocks * block_size - 1)], torch.zeros(1))
+            assert torch.equal(have.cpu(), ref.to(dtype))
+
+
+def test_batch_append_matches_the_oracle(cuda_device):
+    gen = np.random.default_rng(4)
+    blocks, heads, dim, bs = 12, 2, 64, 16
+    tables = torch.from_numpy(gen.permutation(blocks)[:10].astype(np.int64)).view(5, 2)
+    tables[3, 1] = blocks + 4
+    offsets = torch.tensor([0, 17, 31, 20, 40])  # the fourth meets an invalid page, the last is past its table
+    rows = randn(gen, 2, 5, heads, dim).to(torch.bfloat16)
+    want = np.zeros((2, blocks, heads, int4_page_bytes(bs, dim)), dtype=np.uint8)
+    for b in range(3):
+        slot = int(tables[b, offsets[b] // bs]) * bs + int(offsets[b]) % bs
+        for i in range(2):
+            int4_kv.write_row(want[i], bs, slot, rows[i, b])
+    got = torch.zeros(want.shape, dtype=torch.uint8, device="cuda")
+    write_kv_cache_batch_int4(got[0], got[1], tables.cuda(), offsets.cuda(), rows[0].cuda(), rows[1].cuda(), bs,
+                              validate=False)
+    assert np.array_equal(got.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 192, 256])
+def test_decode_head_dims(cuda_device, dtype, dim):
+    decode(np.random.default_rng(dim), dtype, (1, 33, 300), 8, 4, dim, 16)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (7, 1), (8, 1), (9, 1), (20, 1), (6, 2), (24, 8), (4, 4)])
+def test_decode_head_groups(cuda_device, heads, kv_heads):
+    decode(np.random.default_rng(heads), torch.bfloat16, (65, 2, 129), heads, kv_heads, 64, 16)
+
+
+@pytest.mark.parametrize("block_size,lens", [(1, (7, 40)), (5, (64, 3)), (8, (100, 8)), (24, (70, 25)), (48, (96, 47)),
+                                             (256, (513, 1, 300)), (1000, (999, 1001))])
+def test_decode_block_sizes(cuda_device, block_size, lens):
+    decode(np.random.default_rng(block_size), torch.float16, lens, 4, 2, 128, block_size)
+
+
+@pytest.mark.parametrize("lens", [(5000,), (4097, 1, 16, 2500), (31, 32, 33, 63, 64, 65) * 6])
+def test_decode_splits(cuda_device, lens):
+    decode(np.random.default_rng(len(lens)), torch.bfloat16, lens, 16, 8, 64, 16)
+
+
+@pytest.mark.parametrize("scale,q_scale", [(2.0 ** -12, 1.0), (3000.0, 2.0 ** -8), (1.0, 2.0 ** -40), (2.0 ** -9, 2.0 ** 30)])
+def test_decode_extreme_scales(cuda_device, scale, q_scale):
+    decode(np.random.default_rng(9), torch.bfloat16, (40, 700), 8, 2, 64, 16, scale=scale, q_scale=q_scale)
+
+
+def test_decode_of_values_of_very_different_sizes(cuda_device):
+    """The token that takes the weight has tiny values, the others large ones."""
+    gen = np.random.default_rng(10)
+    bs, dim = 16, 64
+    kp, vp = (np.zeros((6, 1, int4_kv.page_bytes(bs, dim)), dtype=np.uint8) for _ in range(2))
+    k, v = randn(gen, 90, 1, dim), randn(gen, 90, 1, dim) * 200
+    query = randn(gen, 1, 2, dim).to(torch.float16)
+    k[3, 0] = query[0, 0].float() * 4
+    v[3] *= 2.0 ** -18
+    slots = torch.arange(90)
+    int4_kv.scatter(kp, bs, slots, k)
+    int4_kv.scatter(vp, bs, slots, v)
+    table, lens = torch.arange(6).view(1, 6), torch.tensor([90])
+    keys, vals = int4_kv.values(kp, bs, dim), int4_kv.values(vp, bs, dim)
+    expected = int4_kv.paged_decode(query, keys, vals, table, lens, bs)
+    actual = paged_attention_int4(query.cuda(), torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(), table.cuda(),
+                                  lens.cuda(), bs)
+    assert_near(actual, expected, query, keys, vals, torch.float16, False)
+
+
+def test_decode_guards(cuda_device):
+    """Invalid pages and lengths: masked tokens, zero rows, nothing read outside."""
+    def spoil(table):
+        table[0].fill_(-1)
+        table[1, 3] = 1 << 40
+        table[3, 0] = -7
+        return table
+
+    actual, _ = decode(np.random.default_rng(11), torch.bfloat16, (65, 300, 0, 17, 1 << 40, -3), 8, 2, 64, 16,
+                       tables=spoil, validate=False, pool_lens=[65, 300, 16, 17, 16, 16])
+    assert torch.isfinite(actual).all() and not actual[0].any() and not actual[2].any()
+    assert not actual[4].any() and not actual[5].any()
+    assert _lib.device_status() == 0
+
+
+def test_decode_ignores_what_lies_behind_the_length(cuda_device):
+    gen = np.random.default_rng(12)
+    bs, dim = 16, 128
+    kp, vp = make_pool(gen, 4, bs, 2, dim), make_pool(gen, 4, bs, 2, dim)
+    query = randn(gen, 1, 4, dim).to(torch.bfloat16).cuda()
+    table, lens = torch.tensor([[2, 0]]).cuda(), torch.tensor([21]).cuda()
+    first = paged_attention_int4(query, torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(), table, lens, bs)
+    for pool in (kp, vp):  # NaN and infinite pairs, other codes, behind position 21 and in unused pages
+        pairs = pool[..., bs * dim // 2:bs * (dim // 2 + 4)].view(np.float16).reshape(4, 2, bs, 2)
+        pairs[0, :, 5:] = np.nan
+        pairs[1], pairs[3] = np.inf, np.nan
+        pool[0, :, 5 * dim // 2:bs * dim // 2] = 0xff
+    again = paged_attention_int4(query, torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(), table, lens, bs)
+    assert torch.equal(first, again)
+
+
+def test_decode_of_a_zeroed_pool_is_zero(cuda_device):
+    pool = torch.zeros(3, 2, int4_page_bytes(16, 64), dtype=torch.uint8, device="cuda")
+    query = torch.ones(1, 4, 64, dtype=torch.float16, device="cuda")
+    out = paged_attention_int4(query, pool, pool.clone(), torch.tensor([[1, 2]]).cuda(), torch.tensor([20]).cuda(), 16)
+    assert not out.any()
+
+
+def test_decode_with_selected_blocks(cuda_device):
+    gen = np.random.default_rng(13)
+    lens = (300, 40, 17)
+    selected = torch.full((3, 2, 6), -1, dtype=torch.int64)
+    selected[0, 0, :4] = torch.tensor([0, 5, 9, 18])
+    selected[0, 1, :6] = torch.tensor([1, 2, 3, 16, 17, 18])
+    selected[1, 0, :3] = torch.tensor([0, 1, 2])
+    selected[1, 1, :1] = torch.tensor([2])
+    selected[2, 0, :1] = torch.tensor([1])  # the other head of request 2 attends nothing
+    actual, _ = decode(gen, torch.bfloat16, lens, 6, 2, 128, 16, selected=selected)
+    assert not actual[2, 3:].any()
+    # every block listed: the attention over the whole table
+    full, blocks = tables_for(gen, [70], 24)
+    kp, vp = make_pool(gen, blocks, 24, 2, 64), make_pool(gen, blocks, 24, 2, 64)
+    args = [randn(gen, 1, 4, 64).to(torch.float16).cuda(), torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(),
+            full.cuda(), torch.tensor([70]).cuda(), 24]
+    all_blocks = torch.arange(3).expand(1, 2, 3).contiguous().cuda()
+    assert torch.equal(paged_attention_int4(*args), paged_attention_int4(*args, selected=all_blocks))
+
+
+def test_decode_is_repeatable_and_independent_of_the_batch(cuda_device):
+    gen = np.random.default_rng(14)
+    table, blocks = tables_for(gen, [2000] * 4, 16)
+    kp, vp = (torch.from_numpy(make_pool(gen, blocks, 16, 2, 64)).cuda() for _ in range(2))
+    query = randn(gen, 4, 8, 64).to(torch.float16).cuda()
+    lens = torch.tensor([2000, 1500, 3, 900]).cuda()
+    first = paged_attention_int4(query, kp, vp, table.cuda(), lens, 16)
+    for _ in range(5):
+        assert torch.equal(first, paged_attention_int4(query, kp, vp, table.cuda(), lens, 16))
+
+
+def test_calls_of_other_shapes_between(cuda_device):
+    """The ticket counters are zero after every call, whatever came before on the stream."""
+    gen = np.random.default_rng(15)
+    cases = []
+    for batch, n in ((2, 3000), (300, 40), (1, 5000), (64, 200), (2, 3000)):
+        table, blocks = tables_for(gen, [n] * batch, 16)
+        pools = [torch.from_numpy(make_pool(gen, min(blocks, 40), 16, 1, 32)).cuda() for _ in range(2)]
+        table = (table % min(blocks, 40)).cuda()
+        cases.append((randn(gen, batch, 2, 32).to(torch.bfloat16).cuda(), *pools, table,
+                      torch.full((batch,), n).cuda(), 16))
+    alone = [paged_attention_int4(*c) for c in cases]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for c, want in zip(cases, alone):
+            assert torch.equal(paged_attention_int4(*c, validate=False), want)
+
+
+def test_decode_on_other_streams_and_in_graphs(cuda_device):
+    """Two graphs captured on one stream are replayed at once on two others, beside eager calls."""
+    gen = np.random.default_rng(16)
+    table, blocks = tables_for(gen, [4000] * 2, 16)
+    kp, vp = (torch.from_numpy(make_pool(gen, blocks, 16, 2, 64)).cuda() for _ in range(2))
+    table = table.cuda()
+    lens = [torch.tensor(x).cuda() for x in ([4000, 3000], [100, 3999])]
+    query = [randn(gen, 2, 8, 64).to(torch.bfloat16).cuda() for _ in range(2)]
+    want = [paged_attention_int4(q, kp, vp, table, n, 16) for q, n in zip(query, lens)]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    graphs, outs = [], []
+    for q, n in zip(query, lens):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(paged_attention_int4(q, kp, vp, table, n, 16, validate=False))
+        graphs.append(graph)
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        eager = paged_attention_int4(query[0], kp, vp, table, lens[0], 16, validate=False)
+        for side, graph in zip(sides, graphs):
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0]) and torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    # new lengths in a captured graph
+    lens[0].copy_(torch.tensor([5, 4000]))
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], paged_attention_int4(query[0], kp, vp, table, lens[0], 16))
+
+
+# ------------------------------------------------------------------ prefill
+
+def prefill(gen, dtype, counts, starts, heads, kv_heads, dim, block_size, *, tables=None, lens=None, extra=0,
+            validate=True, scale=1.0, max_query_len=None):
+    full = [s + c for s, c in zip(starts, counts)]
+    table, blocks = tables_for(gen, [max(1, n) for n in full], block_size)
+    if tables is not None:
+        table = tables(table)
+    kp, vp = make_pool(gen, blocks, block_size, kv_heads, dim, scale), make_pool(gen, blocks, block_size, kv_heads, dim, scale)
+    cu = torch.tensor([0, *np.cumsum(counts)], dtype=torch.int64)
+    starts = torch.tensor(starts, dtype=torch.int64)
+    lens = torch.tensor(full if lens is None else lens, dtype=torch.int64)
+    q = randn(gen, int(cu[-1]) + extra, heads, dim).to(dtype)
+    keys, vals = int4_kv.values(kp, block_size, dim), int4_kv.values(vp, block_size, dim)
+    expected = int4_kv.paged_prefill(q, keys, vals, cu, starts, table, lens, block_size)
+    actual = paged_prefill_attention_int4(q.cuda(), torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(), cu.cuda(),
+                                          starts.cuda(), table.cuda(), lens.cuda(), block_size, validate=validate,
+                                          max_query_len=max_query_len)
+    assert actual.dtype == dtype and actual.shape == q.shape
+    assert_near(actual, expected, q, keys, vals, dtype, True)
+    return actual
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 192, 256])
+def test_prefill_head_dims(cuda_device, dtype, dim):
+    prefill(np.random.default_rng(dim), dtype, (1, 70, 33), (0, 37, 200), 8, 4, dim, 16)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 1), (7, 1), (14, 2), (64, 1), (4, 4)])
+def test_prefill_head_groups(cuda_device, heads, kv_heads):
+    prefill(np.random.default_rng(heads), torch.bfloat16, (40, 5), (100, 0), heads, kv_heads, 64, 16)
+
+
+@pytest.mark.parametrize("block_size,counts,starts", [(1, (9, 20), (3, 0)), (5, (30,), (64,)), (24, (65, 64, 63), (0, 1, 127)),
+                                                      (256, (300, 2), (255, 256)), (16, (0, 17, 0), (5, 1, 9))])
+def test_prefill_block_sizes_and_lengths(cuda_device, block_size, counts, starts):
+    prefill(np.random.default_rng(block_size), torch.float16, counts, starts, 4, 2, 128, block_size)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -12, 2000.0])
+def test_prefill_extreme_scales(cuda_device, scale):
+    prefill(np.random.default_rng(21), torch.bfloat16, (50,), (90,), 4, 2, 64, 16, scale=scale)
+
+
+def test_prefill_growing_steps(cuda_device):
+    """Values whose steps grow along the keys by far more than fp16's range."""
+    gen = np.random.default_rng(22)
+    bs, dim, n = 16, 64, 400
+    kp, vp = (np.zeros((25, 1, int4_kv.page_bytes(bs, dim)), dtype=np.uint8) for _ in range(2))
+    v = randn(gen, n, 1, dim) * torch.exp2(torch.linspace(-16, 13, n))[:, None, None]
+    int4_kv.scatter(kp, bs, torch.arange(n), randn(gen, n, 1, dim))
+    int4_kv.scatter(vp, bs, torch.arange(n), v)
+    keys, vals = int4_kv.values(kp, bs, dim), int4_kv.values(vp, bs, dim)
+    q = randn(gen, n, 2, dim).to(torch.bfloat16)
+    cu, starts, lens = torch.tensor([0, n]), torch.tensor([0]), torch.tensor([n])
+    table = torch.arange(25).view(1, 25)
+    expected = int4_kv.paged_prefill(q, keys, vals, cu, starts, table, lens, bs)
+    actual = paged_prefill_attention_int4(q.cuda(), torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(), cu.cuda(),
+                                          starts.cuda(), table.cuda(), lens.cuda(), bs)
+    # row by row: each has its own range of values (those it sees)
+    for i in range(0, n, 7):
+        assert_near(actual[i:i + 1], expected[i:i + 1], q[i:i + 1], keys, vals.view(-1, 1, dim)[:i + 1],
+                    torch.bfloat16, True)
+
+
+def test_prefill_guards(cuda_device):
+    """Invalid pages, contexts that end early, tokens of no request, a bound below a request's length."""
+    def spoil(table):
+        table[0, 1] = -1
+        table[1].fill_(1 << 33)
+        return table
+
+    actual = prefill(np.random.default_rng(23), torch.bfloat16, (60, 20, 50), (0, 7, 30), 4, 2, 64, 16, tables=spoil,
+                     lens=(60, 27, 60), extra=9, validate=False, max_query_len=10)
+    assert not actual[60:80].any()          # every page of request 1 is invalid
+    assert not actual[110:130].any()        # positions 60..79 of request 2 lie past its context
+    assert not actual[130:].any()           # tokens of no request
+
+
+def test_prefill_matches_decode(cuda_device):
+    """The last token of a prefill and the decode at its position agree to their roundings."""
+    gen = np.random.default_rng(24)
+    table, blocks = tables_for(gen, [200], 16)
+    kp, vp = (torch.from_numpy(make_pool(gen, blocks, 16, 2, 128)).cuda() for _ in range(2))
+    q = randn(gen, 50, 8, 128).to(torch.bfloat16).cuda()
+    cu, starts, lens = (torch.tensor(x).cuda() for x in ([0, 50], [150], [200]))
+    pre = paged_prefill_attention_int4(q, kp, vp, cu, starts, table.cuda(), lens, 16)
+    dec = paged_attention_int4(q[-1:].contiguous(), kp, vp, table.cuda(), lens, 16)
+    assert float((pre[-1:].float() - dec.float()).norm()) <= 2 * 2.0 ** -8 * float(dec.float().norm())
