@@ -44,8 +44,8 @@ struct PageDecodeParams {
     const int64_t* lens;
     const int64_t* selected;  // [batch, kv_heads, take] logical blocks, or null: all
     void* out;
-    float* partial;           // [units + grid][heads][D]
-    float* lse;               // [units + grid][heads], log2
+    float* partial;           // [units + runs][heads][D]
+    float* lse;               // [units + runs][heads], log2
     unsigned int* tickets;    // [units], zero before and after
     int batch, q_heads, kv_heads, group, chunks, heads;  // heads: query heads of a unit's record, min(group, 8)
     int num_blocks, block_size, width, take;
@@ -78,6 +78,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ uint32_t permute_bytes(uint32_t a, uint32_t b, uint32_t sel) {
@@ -119,6 +129,11 @@ __device__ __forceinline__ float column_sum(float x) {
     return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
 
+// The running maximum is raised only when a score exceeds it by more than 2^8, so P <= 2^8 (fp16
+// holds 65504), O is rescaled once or twice a unit, and the maximum over a column's lanes is taken
+// only then: a vote tells.
+constexpr float kMaxSlack = 8.f;
+
 constexpr uint32_t kNibbleMask = 0x000f000fu;  // the low nibbles of two halves
 constexpr float kCodeScale = 16777216.f;       // 2^24: a nibble in the low bits of a half is code 2^-24
 
@@ -133,14 +148,22 @@ constexpr float kCodeScale = 16777216.f;       // 2^24: a nibble in the low bits
 // are of four neighbouring tokens.  The order of the head dims in a dot product
 // is free: lane q4 takes dims q4 D/4 .. of K (whole words of codes) and, for
 // V^T (dims are the M rows), lane g dims g D/8 ..: in each four of them nibble
-// 0 and 2 are rows g and g + 8 of one MMA and nibble 1 and 3 (16 times larger
-// as subnormals) of another.
+// 0 and 2 are rows g and g + 8 of one MMA; another takes the whole bytes, n0 +
+// 16 n1 and n2 + 16 n3 (a byte in the low bits of a half is still a subnormal),
+// and the odd nibbles' sums are the difference at the end: a fifth fewer
+// integer operations than masking both.  For K the odd nibbles are masked out
+// in place (16 times larger as subnormals) and meet a Q scaled by 1/16.
+// A lane first turns the (step, base) pairs of one token into what the scores
+// and the sums need, for the whole warp: done by every lane for its own rows it
+// took a sixth of the tile's instructions.
 template <typename T, int D>
 struct Int4Consumer {
     static constexpr int TT = 32;
     static constexpr int RB = D / 2;                         // bytes of a row's codes
     static constexpr int kRowBytes = RB;                     // ... staged without padding
-    static constexpr int kStageBytes = TT * (2 * RB + 8);    // K codes, V codes, K pairs, V pairs
+    static constexpr int kPairs = TT * 2 * RB;               // stage: K codes, V codes, K pairs, V pairs
+    static constexpr int kStageBytes = kPairs + TT * 8;
+    static constexpr int kScratch = TT * 20;                 // per warp: the tokens' factors
     static constexpr int NW = D / 32;                        // words of K a lane takes of a row
     static constexpr int NH = D / 32;                        // 16-bit runs of V a lane takes of a row
     static constexpr int kPieces = NH;                       // groups of 32 output dims
@@ -151,9 +174,10 @@ struct Int4Consumer {
     uint32_t qb[2 * NW][2];
     float o[2 * NH][4];
     float m[2], l[2], z[2], qsum[2], qscale[2];
-    int g, q4;
+    int g, q4, lane;
 
-    __device__ void setup(int lane) {
+    __device__ void setup(int lane_) {
+        lane = lane_;
         g = lane >> 2;
         q4 = lane & 3;
     }
@@ -185,8 +209,10 @@ struct Int4Consumer {
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                x[i] = __half2float(__float2half_rn(f[8 * w + i] * down));
-                sum += x[i];
+                // fp16 below 2^-14 of the largest element rounds to 2^-24 of it (odd nibbles: 2^-20)
+                const float unit = (i & 1) ? 0.0625f : 1.f;
+                x[i] = __half2float(__float2half_rn(f[8 * w + i] * down * unit));
+                sum += (i & 1) ? x[i] * 16.f : x[i];
             }
             qb[2 * w][0] = Elem<__half>::pack(x[0], x[4]);
             qb[2 * w][1] = Elem<__half>::pack(x[2], x[6]);
@@ -260,76 +286,83 @@ struct Int4Consumer {
         }
     }
 
-    __device__ __forceinline__ void tile(const unsigned char* stage, uint32_t valid, float) {
+    // Raise the maxima to those of the columns, where they exceed them by the slack.
+    __device__ __forceinline__ void raise(const float* top) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float mx = column_max(top[h]);
+            if (mx > m[h] + kMaxSlack) {
+                const float alpha = exp2_fast(m[h] - mx);
+                m[h] = mx;
+                l[h] *= alpha;
+                z[h] *= alpha;
+#pragma unroll
+                for (int x = 0; x < 2 * NH; ++x) {
+                    o[x][h] *= alpha;
+                    o[x][h + 2] *= alpha;
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void tile(const unsigned char* stage, uint32_t valid, float, unsigned char* scratch) {
         const unsigned char* kst = stage;
         const unsigned char* vst = stage + TT * RB;
-        const __half2* kp = reinterpret_cast<const __half2*>(stage + 2 * TT * RB);
-        const __half2* vp = kp + TT;
+        float4* factors = reinterpret_cast<float4*>(scratch);        // [TT]: K step 2^24, K base, log2 V step, 1 / V step
+        float* weights = reinterpret_cast<float*>(scratch + TT * 16);  // [TT]: V base / V step
+        {
+            const __half2* pairs = reinterpret_cast<const __half2*>(stage + kPairs);
+            const float2 k = __half22float2(pairs[lane]), v = __half22float2(pairs[TT + lane]);
+            const float vs = fmaxf(v.x, kInt4StepMin);
+            const float inv = rcp_fast(vs);
+            // a masked token (its codes and pairs are zeros) drops out by log2 P' = -inf
+            factors[lane] = make_float4(fmaxf(k.x, kInt4StepMin) * kCodeScale, k.y,
+                                        (valid >> lane) & 1u ? log2_fast(vs) : -INFINITY, inv);
+            weights[lane] = v.y * inv;
+        }
+        __syncwarp();
         const int row = (g >> 1) + 4 * (g & 1);
-        float t[2][4], rinv[2][2], vbase[2][2];
+        float t[2][4], rinv[2][2], rbase[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r0 = 16 * i + row, r1 = r0 + 8;
             uint32_t k0[NW], k1[NW];
             load_k(kst + r0 * RB + q4 * (RB / 4), k0);
             load_k(kst + r1 * RB + q4 * (RB / 4), k1);
-            float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < NW; ++w) {
                 const uint32_t a[4] = {k0[w] & kNibbleMask, k1[w] & kNibbleMask, (k0[w] >> 8) & kNibbleMask,
                                        (k1[w] >> 8) & kNibbleMask};
-                mma16816<__half>(lo, a, qb[2 * w][0], qb[2 * w][1]);
+                mma16816<__half>(s, a, qb[2 * w][0], qb[2 * w][1]);
                 const uint32_t b[4] = {k0[w] & (kNibbleMask << 4), k1[w] & (kNibbleMask << 4),
                                        (k0[w] >> 8) & (kNibbleMask << 4), (k1[w] >> 8) & (kNibbleMask << 4)};
-                mma16816<__half>(hi, b, qb[2 * w + 1][0], qb[2 * w + 1][1]);
+                mma16816<__half>(s, b, qb[2 * w + 1][0], qb[2 * w + 1][1]);
             }
-            const float2 kp0 = __half22float2(kp[r0]), kp1 = __half22float2(kp[r1]);
-            const float2 vp0 = __half22float2(vp[r0]), vp1 = __half22float2(vp[r1]);
-            const float ks0 = fmaxf(kp0.x, kInt4StepMin) * kCodeScale, ks1 = fmaxf(kp1.x, kInt4StepMin) * kCodeScale;
-            const float vs0 = fmaxf(vp0.x, kInt4StepMin), vs1 = fmaxf(vp1.x, kInt4StepMin);
-            const float lv0 = __log2f(vs0), lv1 = __log2f(vs1);
-            rinv[i][0] = __fdividef(1.f, vs0);
-            rinv[i][1] = __fdividef(1.f, vs1);
-            vbase[i][0] = vp0.y;
-            vbase[i][1] = vp1.y;
-            const bool ok0 = (valid >> r0) & 1u, ok1 = (valid >> r1) & 1u;
+            const float4 f0 = factors[r0], f1 = factors[r1];
+            rinv[i][0] = f0.w;
+            rinv[i][1] = f1.w;
+            rbase[i][0] = weights[r0];
+            rbase[i][1] = weights[r1];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float s0 = fmaf(fmaf(hi[h], 0.0625f, lo[h]), ks0, kp0.y * qsum[h]);
-                const float s1 = fmaf(fmaf(hi[h + 2], 0.0625f, lo[h + 2]), ks1, kp1.y * qsum[h]);
-                t[i][h] = ok0 ? fmaf(s0, qscale[h], lv0) : -INFINITY;
-                t[i][h + 2] = ok1 ? fmaf(s1, qscale[h], lv1) : -INFINITY;
+                t[i][h] = fmaf(fmaf(s[h], f0.x, f0.y * qsum[h]), qscale[h], f0.z);
+                t[i][h + 2] = fmaf(fmaf(s[h + 2], f1.x, f1.y * qsum[h]), qscale[h], f1.z);
             }
         }
-        float alpha[2];
+        float top[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float mx = column_max(fmaxf(fmaxf(t[0][h], t[0][h + 2]), fmaxf(t[1][h], t[1][h + 2])));
-            const float mn = fmaxf(m[h], mx);
-            alpha[h] = mn == -INFINITY ? 1.f : exp2_fast(m[h] - mn);
-            m[h] = mn;
-        }
-        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                l[h] *= alpha[h];
-                z[h] *= alpha[h];
-#pragma unroll
-                for (int x = 0; x < 2 * NH; ++x) {
-                    o[x][h] *= alpha[h];
-                    o[x][h + 2] *= alpha[h];
-                }
-            }
-        }
+        for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(t[0][h], t[0][h + 2]), fmaxf(t[1][h], t[1][h + 2]));
+        if (__any_sync(0xffffffffu, top[0] > m[0] + kMaxSlack || top[1] > m[1] + kMaxSlack)) raise(top);
+        const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};  // 2^(-inf - 0) = 0
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float p[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                p[e] = m[e & 1] == -INFINITY ? 0.f : exp2_fast(t[i][e] - m[e & 1]);
-                const float w = p[e] * rinv[i][e >> 1];
-                l[e & 1] += w;
-                z[e & 1] = fmaf(w, vbase[i][e >> 1], z[e & 1]);
+                p[e] = exp2_fast(t[i][e] - mm[e & 1]);
+                l[e & 1] = fmaf(p[e], rinv[i][e >> 1], l[e & 1]);
+                z[e & 1] = fmaf(p[e], rbase[i][e >> 1], z[e & 1]);
             }
             const uint32_t p01 = Elem<__half>::pack(p[0], p[1]), p23 = Elem<__half>::pack(p[2], p[3]);
             const uint32_t b0 = transpose8x8(p01), b1 = transpose8x8(p23);
@@ -347,10 +380,9 @@ struct Int4Consumer {
             load_v(v + 8 * RB, v + 12 * RB, x1);
 #pragma unroll
             for (int u = 0; u < NH; ++u) {
-                const uint32_t a[4] = {x0[u] & kNibbleMask, (x0[u] >> 8) & kNibbleMask, x1[u] & kNibbleMask,
-                                       (x1[u] >> 8) & kNibbleMask};
-                const uint32_t b[4] = {x0[u] & (kNibbleMask << 4), (x0[u] >> 8) & (kNibbleMask << 4),
-                                       x1[u] & (kNibbleMask << 4), (x1[u] >> 8) & (kNibbleMask << 4)};
+                const uint32_t b[4] = {x0[u] & 0x00ff00ffu, permute_bytes(x0[u], 0u, 0x4341u), x1[u] & 0x00ff00ffu,
+                                       permute_bytes(x1[u], 0u, 0x4341u)};
+                const uint32_t a[4] = {b[0] & kNibbleMask, b[1] & kNibbleMask, b[2] & kNibbleMask, b[3] & kNibbleMask};
                 mma16816<__half>(o[2 * u], a, b0, b1);
                 mma16816<__half>(o[2 * u + 1], b, b0, b1);
                 if constexpr (kTwoTerms) {
@@ -361,16 +393,30 @@ struct Int4Consumer {
         }
     }
 
-    // Piece u of the accumulators times f[h]: element [head][x] for x < 32 is output dim dim_of(u, x).
+    // Piece u of the accumulators times f[h]: element [head % 4][x] for x < 32 is output dim dim_of(u, x).
     __device__ __forceinline__ void put_piece(int u, const float* f, float* dst) const {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const float lo = f[h] * kCodeScale, hi = f[h] * (kCodeScale / 16.f);
-            *reinterpret_cast<float4*>(dst + (2 * q4 + h) * 32 + 4 * g) =
-                make_float4(o[2 * u][h] * lo, o[2 * u + 1][h] * hi, o[2 * u][h + 2] * lo, o[2 * u + 1][h + 2] * hi);
+            const float k = f[h] * kCodeScale;
+            *reinterpret_cast<float4*>(dst + ((2 * q4 + h) & 3) * 32 + 4 * g) =
+                make_float4(o[2 * u][h] * k, high(u, h) * k, o[2 * u][h + 2] * k, high(u, h + 2) * k);
         }
     }
+    // sums of the odd nibbles, from those of the even ones and of the bytes
+    __device__ __forceinline__ float high(int u, int i) const { return (o[2 * u + 1][i] - o[2 * u][i]) * 0.0625f; }
     __device__ static __forceinline__ int dim_of(int u, int x) { return (x >> 2) * (D / 8) + 4 * u + (x & 3); }
+    // The lane's part of head 2 q4 + h: (O + add) * inv into a row of V (fp32 or T).
+    template <typename V> __device__ __forceinline__ void put_row(int h, float add, float inv, V* row) const {
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) {
+            const float f[4] = {fmaf(o[2 * u][h], kCodeScale, add) * inv, fmaf(high(u, h), kCodeScale, add) * inv,
+                                fmaf(o[2 * u][h + 2], kCodeScale, add) * inv,
+                                fmaf(high(u, h + 2), kCodeScale, add) * inv};
+            V* dst = row + g * (D / 8) + 4 * u;
+            if constexpr (sizeof(V) == 4) *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+            else *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<V>::pack(f[0], f[1]), Elem<V>::pack(f[2], f[3]));
+        }
+    }
 };
 
 // 16-bit pool, 16 tokens a tile; K and V rows are padded by 16 bytes so that
@@ -381,7 +427,9 @@ struct Wide16Consumer {
     static constexpr int TT = 16;
     static constexpr int RB = 2 * D;
     static constexpr int kRowBytes = RB + 16;
+    static constexpr int kPairs = 0;
     static constexpr int kStageBytes = TT * 2 * kRowBytes;
+    static constexpr int kScratch = 0;
     static constexpr int KSTEPS = D / 16;
     static constexpr int kPieces = D / 32;
 
@@ -411,7 +459,24 @@ struct Wide16Consumer {
         l[0] = l[1] = z[0] = z[1] = 0.f;
     }
 
-    __device__ __forceinline__ void tile(const unsigned char* stage, uint32_t valid, float scale_log2) {
+    __device__ __forceinline__ void raise(const float* top) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float mx = column_max(top[h]);
+            if (mx > m[h] + kMaxSlack) {
+                const float alpha = exp2_fast(m[h] - mx);
+                m[h] = mx;
+                l[h] *= alpha;
+#pragma unroll
+                for (int x = 0; x < KSTEPS; ++x) {
+                    o[x][h] *= alpha;
+                    o[x][h + 2] *= alpha;
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void tile(const unsigned char* stage, uint32_t valid, float scale_log2, unsigned char*) {
         const uint32_t base = smem_addr(stage);
         float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -425,28 +490,13 @@ struct Wide16Consumer {
         s[1] = ok0 ? (s[1] + s2[1]) * scale_log2 : -INFINITY;
         s[2] = ok1 ? (s[2] + s2[2]) * scale_log2 : -INFINITY;
         s[3] = ok1 ? (s[3] + s2[3]) * scale_log2 : -INFINITY;
-        float alpha[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float mn = fmaxf(m[h], column_max(fmaxf(s[h], s[h + 2])));
-            alpha[h] = mn == -INFINITY ? 1.f : exp2_fast(m[h] - mn);
-            m[h] = mn;
-        }
-        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                l[h] *= alpha[h];
-#pragma unroll
-                for (int x = 0; x < KSTEPS; ++x) {
-                    o[x][h] *= alpha[h];
-                    o[x][h + 2] *= alpha[h];
-                }
-            }
-        }
+        const float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+        if (__any_sync(0xffffffffu, top[0] > m[0] + kMaxSlack || top[1] > m[1] + kMaxSlack)) raise(top);
+        const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};  // 2^(-inf - 0) = 0
         float p[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            p[e] = m[e & 1] == -INFINITY ? 0.f : exp2_fast(s[e] - m[e & 1]);
+            p[e] = exp2_fast(s[e] - mm[e & 1]);
             l[e & 1] += p[e];
         }
         const uint32_t p01 = Elem<T>::pack(p[0], p[1]), p23 = Elem<T>::pack(p[2], p[3]);
@@ -468,7 +518,7 @@ struct Wide16Consumer {
     __device__ __forceinline__ void put_piece(int u, const float* f, float* dst) const {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float* row = dst + (2 * q4 + h) * 32 + g;
+            float* row = dst + ((2 * q4 + h) & 3) * 32 + g;
             row[0] = o[2 * u][h] * f[h];
             row[8] = o[2 * u][h + 2] * f[h];
             row[16] = o[2 * u + 1][h] * f[h];
@@ -476,35 +526,102 @@ struct Wide16Consumer {
         }
     }
     __device__ static __forceinline__ int dim_of(int u, int x) { return 32 * u + x; }
+    template <typename V> __device__ __forceinline__ void put_row(int h, float add, float inv, V* row) const {
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k) {
+            row[16 * k + g] = Elem<V>::from_float((o[k][h] + add) * inv);
+            row[16 * k + g + 8] = Elem<V>::from_float((o[k][h + 2] + add) * inv);
+        }
+    }
 };
 
 // ------------------------------------------------------------------ the kernel
 template <typename Consumer, bool INT4> struct PageShape {
     static constexpr int kWarps = INT4 ? 8 : 4;
-    static constexpr int kStages = INT4 ? 2 : 3;
+    static constexpr int kStages = 3;
     static constexpr int kThreads = kWarps * 32;
-    static constexpr int kRing = kWarps * kStages * Consumer::kStageBytes;
-    static constexpr int kPiece = kWarps * 8 * 32 * 4;  // one piece of every warp's accumulators
-    // ring | piece | warps' (m, l, z) of 8 heads | stage masks | tile prefix
-    static constexpr int kFixed = kRing + kPiece + kWarps * 8 * 3 * 4 + kWarps * kStages * 4;
+    static constexpr int kStage = Consumer::kStageBytes + 16;  // and the mask of its tokens
+    static constexpr int kPiece = kWarps * 4 * 32 * 4;         // one piece of every warp's accumulators, four heads
+    static constexpr int kWork = kWarps * Consumer::kScratch > kPiece ? kWarps * Consumer::kScratch : kPiece;
+    // rings | consumers' scratch, or a piece | warps' (m, l, z) of 8 heads | slices | prefix of tiles
+    static constexpr int kScratch = kWarps * kStages * kStage;
+    static constexpr int kStats = kScratch + kWork;
+    static constexpr int kSlices = kStats + kWarps * 8 * 3 * 4;
+    static constexpr int kPrefix = kSlices + kWarps * 16 * 16;
+    static constexpr int kBytes = kPrefix + (kThreads + 4) * 4;
 };
 
-// A place in the list of tiles: tile j of unit ul (of request b).
+// A place in the list of tiles: tile j of unit ul of request b, whose units have `tiles` tiles each
+// and whose list has `len` tokens.
 struct TileCursor {
-    int b, ul, j, tiles;  // tiles: of each unit of request b
+    int b, ul, j, tiles, len;
 };
 
-template <typename T, int D, typename Consumer, bool INT4, bool SELECTED>
-__global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, (INT4 ? D <= 128 : D <= 128) ? 2 : 1)
+// 16 tokens of one page: where their codes (rows) start in the pool, their (step, base) pairs
+// relative to that, and which of them exist.
+struct __align__(16) PageSlice {
+    int64_t at;
+    int pairs;
+    uint32_t mask;
+};
+
+constexpr int kMostPartials = 3;  // of a unit that warps work on alone (measured: see page_decode_kernel)
+
+// Joins n partials of a unit, in their order, into its output rows: `threads` threads share the
+// heads x D elements, four each at a time.  Up to four partials are loaded at once.
+template <typename T, int D>
+__device__ void join_partials(const PageDecodeParams& p, int64_t first, int n, int heads, int64_t qh0, int thread,
+                              int threads) {
+    constexpr int AT_ONCE = 4;
+#pragma unroll 2
+    for (int x = thread; x < heads * (D / 4); x += threads) {
+        const int head = x / (D / 4), d = (x - head * (D / 4)) * 4;
+        const float* lse = p.lse + first * p.heads + head;
+        const float4* part = reinterpret_cast<const float4*>(p.partial + (first * p.heads + head) * D + d);
+        float mx = -INFINITY, sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = 0; k0 < n; k0 += AT_ONCE) {
+            float e[AT_ONCE];
+            float4 v[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const int64_t at = min(k0 + k, n - 1);
+                e[k] = __ldcg(lse + at * p.heads);
+                v[k] = __ldcg(part + at * p.heads * (D / 4));
+                if (k0 + k >= n) e[k] = -INFINITY;
+            }
+            float top = mx;
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, e[k]);
+            const float keep = mx == -INFINITY ? 0.f : exp2_fast(mx - top);
+            sum *= keep;
+            acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const float w = e[k] == -INFINITY ? 0.f : exp2_fast(e[k] - top);
+                sum += w;
+                acc = make_float4(fmaf(w, v[k].x, acc.x), fmaf(w, v[k].y, acc.y), fmaf(w, v[k].z, acc.z),
+                                  fmaf(w, v[k].w, acc.w));
+            }
+            mx = top;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (qh0 + head) * D + d) =
+            make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
+    }
+}
+
+// ALIGNED: block_size is a multiple of 16, so that a slice of 16 tokens lies in one page.
+template <typename T, int D, typename Consumer, bool INT4, bool SELECTED, bool ALIGNED>
+__global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 ? 2 : 1)
     page_decode_kernel(const PageDecodeParams p) {
     using Shape = PageShape<Consumer, INT4>;
-    constexpr int TT = Consumer::TT, W = Shape::kWarps, NS = Shape::kStages, RB = Consumer::RB;
+    constexpr int TT = Consumer::TT, W = Shape::kWarps, NS = Shape::kStages, RB = Consumer::RB, STAGE = Shape::kStage;
     extern __shared__ __align__(128) unsigned char smem[];
-    float* piece = reinterpret_cast<float*>(smem + Shape::kRing);
-    float* stats = reinterpret_cast<float*>(smem + Shape::kRing + Shape::kPiece);  // [3][W][8]
-    uint32_t* masks = reinterpret_cast<uint32_t*>(stats + 3 * W * 8);              // [W][NS]
-    int* prefix = reinterpret_cast<int*>(masks + W * NS);                          // [B + 1] tiles per unit
-    __shared__ int warp_sums[W];
+    float* piece = reinterpret_cast<float*>(smem + Shape::kScratch);
+    float* stats = reinterpret_cast<float*>(smem + Shape::kStats);  // [3][W][8]
+    int* prefix = reinterpret_cast<int*>(smem + Shape::kPrefix);    // [threads + 1]: tiles before a thread's requests
+    __shared__ int warp_sums[W], warp_most[W];
     __shared__ int last_ticket;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int B = p.batch, U = p.kv_heads * p.chunks;
@@ -526,16 +643,23 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, (INT4 ? D
         }
         return (len + TT - 1) / TT;
     };
-    // ---- exclusive prefix of the requests' tile counts
+    // ---- exclusive prefix of the tile counts: a thread has `per` requests (one, for a batch of up to
+    // W * 32), and those within a thread's are counted again where needed, so any batch fits
+    const int per = (B + W * 32 - 1) / (W * 32);
     {
-        const int per = (B + W * 32 - 1) / (W * 32);
         const int lo = min(B, tid * per), hi = min(B, lo + per);
-        int sum = 0;
+        int sum = 0, most = 0;
         for (int i = lo; i < hi; ++i) {
             const int n = tiles_of(usable(i));
-            prefix[i] = n;
             sum += n;
+            most = max(most, n);
+            if (n == 0 && i % gridDim.x == blockIdx.x)  // nothing to attend: zeros
+                for (int x = 0; x < p.q_heads * D; x += 8)
+                    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)i * p.q_heads * D + x) =
+                        make_uint4(0u, 0u, 0u, 0u);
         }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) warp_most[warp] = most;
         int incl = sum;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -546,38 +670,44 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, (INT4 ? D
         __syncthreads();
         int run = incl - sum;
         for (int w = 0; w < warp; ++w) run += warp_sums[w];
-        for (int i = lo; i < hi; ++i) {
-            const int n = prefix[i];
-            prefix[i] = run;
-            run += n;
-        }
-        if (tid == W * 32 - 1) prefix[B] = run;
+        prefix[tid] = run;
+        if (tid == W * 32 - 1) prefix[W * 32] = run + sum;
         __syncthreads();
     }
-    // ---- rows of requests with nothing to attend are zeros
-    for (int b = blockIdx.x; b < B; b += gridDim.x)
-        if (prefix[b + 1] == prefix[b])
-            for (int i = tid; i < p.q_heads * D; i += W * 32)
-                static_cast<T*>(p.out)[(int64_t)b * p.q_heads * D + i] = Elem<T>::from_float(0.f);
-    // ---- this CTA's run of tiles
-    const int64_t total = (int64_t)prefix[B] * U;
-    const int64_t most = (total + p.min_tiles - 1) / p.min_tiles;
-    const int64_t G = most < gridDim.x ? most : gridDim.x;
-    if (blockIdx.x >= G) return;
-    const int64_t t0 = blockIdx.x * total / G, t1 = (blockIdx.x + 1) * total / G;
-    if (t0 >= t1) return;
+    // ---- teams and their runs of tiles.  A team is the CTA, whose warps take the tiles of its run in
+    // turn and join at the end of each unit, or a single warp with a run of its own: no barrier, an
+    // eighth of the joins, but a unit is then cut into as many partials as warps share it.  Warps
+    // where that is at most kMostPartials; both figures come from the lengths, so all CTAs agree.
+    const int64_t total = (int64_t)prefix[W * 32] * U;
+    int longest = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) longest = max(longest, warp_most[w]);
+    const bool alone = (int64_t)longest * gridDim.x * W <= kMostPartials * total;
+    const int TW = alone ? 1 : W, rank = alone ? 0 : warp;  // warps of the team, and this one's place
+    const int64_t team = alone ? (int64_t)blockIdx.x * W + warp : blockIdx.x;
+    int64_t G = (int64_t)gridDim.x * (alone ? W : 1);  // runs
+    G = min(G, alone ? total : (total + p.min_tiles - 1) / p.min_tiles);  // every run has a tile
+    if (team >= G) return;
+    const int64_t t0 = team * total / G;
+    const int run = (int)((team + 1) * total / G - t0);  // the team's tiles; its warp r takes tiles r, r + TW, ...
 
     auto cursor_at = [&](int64_t t) -> TileCursor {
-        const int64_t x = t / U;  // the request whose tiles [prefix * U, ...) hold t
-        int lo = 0, hi = B - 1;
+        const int64_t x = t / U;  // tiles of the requests before (and of the own one's units, divided)
+        int lo = 0, hi = W * 32 - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (prefix[mid] <= x) lo = mid; else hi = mid - 1;
         }
         TileCursor c;
-        c.b = lo;
-        c.tiles = prefix[lo + 1] - prefix[lo];
-        const int in = (int)(t - (int64_t)prefix[lo] * U);
+        c.b = lo * per;
+        int64_t before = prefix[lo];
+        for (;; ++c.b) {
+            c.len = usable(c.b);
+            c.tiles = tiles_of(c.len);
+            if (x < before + c.tiles || c.b == B - 1) break;
+            before += c.tiles;
+        }
+        const int in = (int)(t - before * U);
         c.ul = in / c.tiles;
         c.j = in - c.ul * c.tiles;
         return c;
@@ -590,261 +720,340 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, (INT4 ? D
                 c.ul = 0;
                 do {
                     if (++c.b >= B) return;
-                    c.tiles = prefix[c.b + 1] - prefix[c.b];
+                    c.len = usable(c.b);
+                    c.tiles = tiles_of(c.len);
                 } while (c.tiles == 0);
             }
         }
     };
 
-    // ---- the warp's copies.  Two look-ups run ahead of them, each one tile further: the listed block
-    // of a token (lane r holds token r of the tile), then its page.
-    unsigned char* ring = smem + warp * NS * Consumer::kStageBytes;
+    // ---- the warp's copies: tile k of the warp is tile rank + k TW of the run.
+    // Aligned: lane x < 16 looks up slice x % SPT of tile x / SPT of a batch of TPB tiles, whose slices lie
+    // in shared memory while the next batch is looked up in two steps (listed block, then page), so that
+    // no step waits for a load of its own.  Otherwise lane r looks up token r of the next tile.
+    unsigned char* ring = smem + warp * NS * STAGE;
     const uint32_t ring_addr = smem_addr(ring);
-    uint32_t* my_masks = masks + warp * NS;
-    TileCursor ahead = cursor_at(t0);
-    int64_t t_list = t0 + warp;  // the next tile to look up
-    if (t_list < t1) advance(ahead, warp);
-    int64_t list_block = -1;     // listed block, and where the token lies
-    int list_off = 0, list_b = 0, list_kvh = 0, list_len = 0, len_b = -1, len_now = 0;
-    int page = -1, page_off = 0, page_kvh = 0;
-    int64_t t_copy = t0 + warp;  // the next tile to copy
-
+    const int mine = run > rank ? (run - rank + TW - 1) / TW : 0;
+    constexpr int SPT = TT / 16, TPB = 16 / SPT;
+    constexpr int CPR = RB / 16;  // 16-byte pieces of a row
+    PageSlice* slices = reinterpret_cast<PageSlice*>(smem + Shape::kSlices) + warp * 16;
+    const int in_tile = ALIGNED ? (lane % SPT) * 16 : (TT == 32 ? lane : lane & 15);  // this lane's first token of the tile
+    int look_k = ALIGNED ? (lane & 15) / SPT : 0;                                     // and its tile, of the warp's
+    TileCursor look = {0, 0, 0, 0, 0};
+    if (look_k < mine) look = cursor_at(t0 + rank + (int64_t)look_k * TW);
+    int64_t block = -1;  // looked up: the listed block
+    int page = -1;       // and its page
+    auto place = [&](int& e, int& off) {  // of this lane's token in the list: entry and row
+        const int v = look.j * TT + in_tile;
+        e = (int)(((uint64_t)(uint32_t)v * p.bs_magic) >> 42);
+        off = v - e * p.block_size;
+    };
+    auto kv_head = [&]() { return p.chunks == 1 ? look.ul : look.ul / p.chunks; };
     auto look_block = [&]() {
-        list_block = -1;
-        if (t_list < t1) {
-            if (ahead.b != len_b) {
-                len_b = ahead.b;
-                len_now = usable(len_b);
-            }
-            list_b = ahead.b;
-            list_len = len_now;
-            list_kvh = ahead.ul / p.chunks;
-            const int v = ahead.j * TT + (TT == 32 ? lane : lane & 15);
-            const int e = (int)(((uint64_t)v * p.bs_magic) >> 42);
-            list_off = v - e * p.block_size;
+        block = -1;
+        if (look_k < mine) {
+            int e, off;
+            place(e, off);
             if (SELECTED) {
-                if (e < p.take) list_block = p.selected[((int64_t)list_b * p.kv_heads + list_kvh) * p.take + e];
+                if (e < p.take) block = p.selected[((int64_t)look.b * p.kv_heads + kv_head()) * p.take + e];
             } else {
-                list_block = e;
+                block = e;
             }
-            t_list += W;
-            if (t_list < t1) advance(ahead, W);
         }
     };
     auto look_page = [&]() {
         page = -1;
-        page_off = list_off;
-        page_kvh = list_kvh;
-        if (list_block >= 0 && list_block < p.width && list_block * p.block_size + list_off < list_len) {
-            const int64_t id = p.tables[(int64_t)list_b * p.width + list_block];
-            page = id >= 0 && id < p.num_blocks ? (int)id : -1;
+        if (block >= 0 && block < p.width) {
+            int e, off;
+            place(e, off);
+            if ((int)block * p.block_size + off < look.len) {
+                const int64_t id = p.tables[(int64_t)look.b * p.width + block];
+                if (id >= 0 && id < p.num_blocks) page = (int)id;
+            }
         }
     };
-    auto copy_tile = [&](int slot) {
-        if (t_copy < t1) {
-            const uint32_t dst = ring_addr + slot * Consumer::kStageBytes;
-            const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0);
-            if (lane == 0) my_masks[slot] = valid;
-            const int64_t head = (int64_t)page_kvh * p.head_stride;
-            constexpr int CPR = RB / 16;  // 16-byte pieces of a row
+    auto look_on = [&](int by) {
+        look_k += by;
+        if (look_k < mine) advance(look, by * TW);
+    };
+    auto keep_batch = [&]() {
+        PageSlice s;
+        s.at = 0;
+        s.pairs = 0;
+        s.mask = 0;
+        if (page >= 0) {
+            int e, off;
+            place(e, off);
+            const int left = look.len - ((int)block * p.block_size + off);
+            s.mask = left >= 16 ? 0xffffu : (1u << left) - 1u;
+            s.at = (int64_t)page * p.page_stride + (int64_t)kv_head() * p.head_stride + off * p.row_stride;
+            if (INT4) s.pairs = p.block_size * RB + off * 4 - off * RB;
+        }
+        __syncwarp();
+        if (lane < 16) slices[lane] = s;
+        __syncwarp();
+    };
+    // a whole slice of K or of V is PIECES pieces a lane, when those divide evenly
+    constexpr bool EVEN = CPR % 2 == 0 && (INT4 || 32 % CPR == 0);
+    constexpr int PIECES = CPR / 2, CPR_ = 32 % CPR == 0 ? CPR : 32;
+    const int64_t lane_from = INT4 ? lane * 16 : (int64_t)(lane / CPR_) * p.row_stride + lane % CPR_ * 16;
+    const uint32_t lane_to = ring_addr + (INT4 ? lane * 16 : lane / CPR_ * Consumer::kRowBytes + lane % CPR_ * 16);
+    const unsigned char* k_lane = p.kc + lane_from;
+    const int64_t v_from_k = (int64_t)(reinterpret_cast<uintptr_t>(p.vc) - reinterpret_cast<uintptr_t>(p.kc));
+    int copied = 0;          // tiles copied
+    uint32_t copy_at = 0;    // stage of the next one, as an offset in the ring
+    auto copy_aligned = [&]() {
+        const int i = copied % TPB;
+        if (i == 0 && copied) keep_batch();
+        if (i == 0) {
+            look_on(TPB);
+            look_block();
+        }
+        if (i == TPB / 2) look_page();
+        uint32_t valid = 0;
 #pragma unroll
-            for (int c0 = 0; c0 < TT * CPR; c0 += 32) {
-                const int c = c0 + lane;
-                const int r = min(c / CPR, TT - 1), x = c - (c / CPR) * CPR;
-                const int pg = __shfl_sync(0xffffffffu, page, r), off = __shfl_sync(0xffffffffu, page_off, r);
-                if (TT * CPR % 32 == 0 || c < TT * CPR) {
-                    const int64_t at = pg < 0 ? 0 : pg * p.page_stride + head + off * p.row_stride + x * 16;
-                    const uint32_t n = pg < 0 ? 0u : 16u;
-                    copy16(dst + r * Consumer::kRowBytes + x * 16, p.kc + at, n);
-                    copy16(dst + (TT + r) * Consumer::kRowBytes + x * 16, p.vc + at, n);
+        for (int s = 0; s < SPT; ++s) {
+            const PageSlice sl = slices[i * SPT + s];
+            valid |= sl.mask << (16 * s);
+            const unsigned char* ks = k_lane + sl.at;
+            const unsigned char* vs = ks + v_from_k;
+            const uint32_t to = lane_to + copy_at + 16 * s * Consumer::kRowBytes;
+            if (EVEN && sl.mask == 0xffffu) {  // the usual slice: whole
+#pragma unroll
+                for (int x = 0; x < PIECES; ++x) {
+                    const int64_t step = INT4 ? x * 512 : x * (32 / CPR_) * p.row_stride;
+                    const uint32_t at = to + (INT4 ? x * 512 : x * (32 / CPR_) * Consumer::kRowBytes);
+                    copy16(at, ks + step, 16u);
+                    copy16(at + TT * Consumer::kRowBytes, vs + step, 16u);
+                }
+            } else {  // 16 CPR pieces of K, then as many of V
+#pragma unroll 1
+                for (int x = 0; x < CPR; ++x) {
+                    const int c = x * 32 + lane;
+                    const bool is_v = c >= 16 * CPR;
+                    const int in = is_v ? c - 16 * CPR : c;
+                    const int row = in / CPR;
+                    const bool on = (sl.mask >> row) & 1u;
+                    const int64_t from = on ? (int64_t)row * p.row_stride + (in - row * CPR) * 16 : 0;
+                    copy16(ring_addr + copy_at + ((is_v ? TT : 0) + 16 * s + row) * Consumer::kRowBytes + (in - row * CPR) * 16,
+                           (is_v ? p.vc : p.kc) + sl.at + from, on ? 16u : 0u);
                 }
             }
-            if (INT4) {
-                const int64_t at =
-                    page < 0 ? 0 : page * p.page_stride + head + (int64_t)p.block_size * RB + page_off * 4;
-                copy4(dst + 2 * TT * RB + lane * 4, p.kc + at, page < 0 ? 0u : 4u);
-                copy4(dst + 2 * TT * RB + TT * 4 + lane * 4, p.vc + at, page < 0 ? 0u : 4u);
+        }
+        if (INT4 && lane < 8 * SPT) {  // pairs: 64 bytes of K and of V a slice
+            const PageSlice sl = slices[i * SPT + (lane >> 3)];
+            const int x = lane & 3, have = __popc(sl.mask) * 4 - x * 16, left = min(16, max(0, have));
+            const unsigned char* src = p.kc + ((lane & 4) ? v_from_k : 0) + sl.at + sl.pairs + (left ? x * 16 : 0);
+            copy16(ring_addr + copy_at + Consumer::kPairs + ((lane & 4) ? TT * 4 : 0) + (lane >> 3) * 64 + x * 16, src,
+                   (uint32_t)left);
+        }
+        if (lane == 0) *reinterpret_cast<uint32_t*>(ring + copy_at + Consumer::kStageBytes) = valid;
+    };
+    auto copy_rows = [&]() {
+        const uint32_t dst = ring_addr + copy_at;
+        int e, page_off;
+        place(e, page_off);
+        const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) *reinterpret_cast<uint32_t*>(ring + copy_at + Consumer::kStageBytes) = valid;
+        const int64_t head = (int64_t)kv_head() * p.head_stride;
+#pragma unroll
+        for (int c0 = 0; c0 < TT * CPR; c0 += 32) {
+            const int c = c0 + lane;
+            const int r = min(c / CPR, TT - 1), x = c - (c / CPR) * CPR;
+            const int pg = __shfl_sync(0xffffffffu, page, r), off = __shfl_sync(0xffffffffu, page_off, r);
+            if (TT * CPR % 32 == 0 || c < TT * CPR) {
+                const int64_t at = pg < 0 ? 0 : pg * p.page_stride + head + off * p.row_stride + x * 16;
+                const uint32_t n = pg < 0 ? 0u : 16u;
+                copy16(dst + r * Consumer::kRowBytes + x * 16, p.kc + at, n);
+                copy16(dst + (TT + r) * Consumer::kRowBytes + x * 16, p.vc + at, n);
             }
-            t_copy += W;
+        }
+        if (INT4) {
+            const int64_t at = page < 0 ? 0 : page * p.page_stride + head + (int64_t)p.block_size * RB + page_off * 4;
+            copy4(dst + Consumer::kPairs + lane * 4, p.kc + at, page < 0 ? 0u : 4u);
+            copy4(dst + Consumer::kPairs + TT * 4 + lane * 4, p.vc + at, page < 0 ? 0u : 4u);
+        }
+        look_on(1);
+        look_block();
+        look_page();
+    };
+    auto copy_tile = [&]() {
+        if (copied < mine) {
+            if constexpr (ALIGNED) copy_aligned();
+            else copy_rows();
+            ++copied;
+            copy_at = copy_at == (NS - 1) * STAGE ? 0 : copy_at + STAGE;
         }
         copy_commit();
     };
     look_block();
     look_page();
-    look_block();
-#pragma unroll
-    for (int s = 0; s < NS - 1; ++s) {
-        copy_tile(s);
-        look_page();
-        look_block();
-    }
+    if constexpr (ALIGNED) keep_batch();
+#pragma unroll 1
+    for (int s = 0; s < NS - 1; ++s) copy_tile();
 
     Consumer c;
     c.setup(lane);
-    int slot = 0;
-    int64_t t = t0 + warp;
+    unsigned char* scratch = smem + Shape::kScratch + warp * Consumer::kScratch;
+    uint32_t stage = 0;
+    int t = rank;  // the warp's next tile, of the run
     TileCursor seg = cursor_at(t0);
-    for (int64_t lo = t0; lo < t1;) {
-        // ---- one unit's tiles in this CTA's run: [lo, hi)
-        const int64_t unit_lo = (int64_t)prefix[seg.b] * U + (int64_t)seg.ul * seg.tiles, unit_hi = unit_lo + seg.tiles;
-        const int64_t hi = unit_hi < t1 ? unit_hi : t1;
+    for (int done = 0; done < run;) {
+        // ---- one unit's tiles in the team's run: [done, end)
+        const int end = min(run, done + seg.tiles - seg.j);
         const int kvh = seg.ul / p.chunks, chunk = seg.ul - kvh * p.chunks;
         const int heads = min(8, p.group - 8 * chunk);
         const int64_t qh0 = (int64_t)seg.b * p.q_heads + kvh * p.group + 8 * chunk;
         c.begin(static_cast<const T*>(p.q) + qh0 * D, heads, p.scale_log2);
-        for (; t < hi; t += W) {
+        for (; t < end; t += TW) {
             copy_wait<NS - 2>();
             __syncwarp();  // the stage is whole, and the one filled next has been read by every lane
-            copy_tile(slot == 0 ? NS - 1 : slot - 1);
-            look_page();
-            look_block();
-            c.tile(ring + slot * Consumer::kStageBytes, my_masks[slot], p.scale_log2);
-            slot = slot + 1 == NS ? 0 : slot + 1;
+            copy_tile();
+            c.tile(ring + stage, *reinterpret_cast<const uint32_t*>(ring + stage + Consumer::kStageBytes), p.scale_log2,
+                   scratch);
+            stage = stage == (NS - 1) * STAGE ? 0 : stage + STAGE;
         }
-        // ---- join the warps: common maximum, then sums in the order of the warps
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float L = column_sum(c.l[h]), Z = column_sum(c.z[h]);
-            if (lane < 4) {
-                stats[warp * 8 + 2 * c.q4 + h] = c.m[h];
-                stats[(W + warp) * 8 + 2 * c.q4 + h] = L;
-                stats[(2 * W + warp) * 8 + 2 * c.q4 + h] = Z;
-            }
-        }
-        __syncthreads();
-        auto joined_max = [&](int head) {
-            float mx = stats[head];
-#pragma unroll
-            for (int w = 1; w < W; ++w) mx = fmaxf(mx, stats[w * 8 + head]);
-            return mx;
-        };
-        float f[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float mx = joined_max(2 * c.q4 + h);
-            f[h] = c.m[h] == -INFINITY ? 0.f : exp2_fast(c.m[h] - mx);
-        }
-        const bool whole = lo == unit_lo && hi == unit_hi;
+        const bool whole = seg.j == 0 && end - done == seg.tiles;
         const int64_t unit = (int64_t)seg.b * U + seg.ul;
-        const int64_t record = unit + blockIdx.x;  // grows by at least one from segment to segment
-        // W * 32 threads sum 8 x 32 elements a piece
-        constexpr int PER = 256 / (W * 32);
-        float inv[PER], zj[PER];
+        const int64_t record = unit + team;  // grows by at least one from segment to segment
+        const int64_t unit_lo = t0 + done - seg.j;
+        // runs that hold the unit's first and last tile
+        auto owner = [&](int64_t x) { return (int)(((x + 1) * G + total - 1) / total) - 1; };
+        if (alone) {
 #pragma unroll
-        for (int r = 0; r < PER; ++r) {
-            const int head = (tid + r * W * 32) >> 5;
-            const float mx = joined_max(head);
-            float L = 0.f, Z = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float mw = stats[w * 8 + head];
-                const float fw = mw == -INFINITY ? 0.f : exp2_fast(mw - mx);
-                L = fmaf(stats[(W + w) * 8 + head], fw, L);
-                Z = fmaf(stats[(2 * W + w) * 8 + head], fw, Z);
-            }
-            inv[r] = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // NaN stays
-            zj[r] = Z;
-            if (!whole && lane == 0 && head < heads)
-                p.lse[record * p.heads + head] = L == 0.f ? -INFINITY : mx + log2f(L);
-        }
-        for (int u = 0; u < Consumer::kPieces; ++u) {
-            if (u) __syncthreads();
-            c.put_piece(u, f, piece + warp * 256);
-            __syncthreads();
-#pragma unroll
-            for (int r = 0; r < PER; ++r) {
-                const int head = (tid + r * W * 32) >> 5;
+            for (int h = 0; h < 2; ++h) {
+                const float L = column_sum(c.l[h]), Z = column_sum(c.z[h]);
+                const int head = 2 * c.q4 + h;
+                const float inv = L == 0.f ? 0.f : 1.f / L;
                 if (head < heads) {
-                    float sum = zj[r];
-#pragma unroll
-                    for (int w = 0; w < W; ++w) sum += piece[w * 256 + head * 32 + lane];
-                    const int d = Consumer::dim_of(u, lane);
-                    if (whole)
-                        static_cast<T*>(p.out)[(qh0 + head) * D + d] = Elem<T>::from_float(sum * inv[r]);
-                    else
-                        p.partial[(record * p.heads + head) * D + d] = sum * inv[r];
-                }
-            }
-        }
-        if (!whole) {
-            // ---- the CTA that takes the unit's last ticket joins its partials
-            auto owner = [&](int64_t x) { return (int)(((x + 1) * G + total - 1) / total) - 1; };
-            const int c0 = owner(unit_lo), c1 = owner(unit_hi - 1);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                unsigned int old;
-                asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;"
-                             : "=r"(old) : "l"(p.tickets + unit), "r"((unsigned int)(c1 - c0)) : "memory");
-                last_ticket = old == (unsigned int)(c1 - c0);
-            }
-            __syncthreads();
-            if (last_ticket) {
-                __threadfence();
-                const int n = c1 - c0 + 1;
-                const int64_t first = unit + c0;
-                for (int x = tid; x < heads * D; x += W * 32) {
-                    const int head = x / D, d = x - head * D;
-                    const float* lse = p.lse + first * p.heads + head;
-                    const float* part = p.partial + (first * p.heads + head) * D + d;
-                    float mx = -INFINITY, sum = 0.f, acc = 0.f;
-                    for (int k0 = 0; k0 < n; k0 += 8) {
-                        float e[8], v[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const bool in = k0 + k < n;
-                            e[k] = in ? __ldcg(lse + (int64_t)(k0 + k) * p.heads) : -INFINITY;
-                            v[k] = in ? __ldcg(part + (int64_t)(k0 + k) * p.heads * D) : 0.f;
-                        }
-                        float top = mx;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) top = fmaxf(top, e[k]);
-                        const float keep = mx == -INFINITY ? 0.f : exp2_fast(mx - top);
-                        sum *= keep;
-                        acc *= keep;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const float w = e[k] == -INFINITY ? 0.f : exp2_fast(e[k] - top);
-                            sum += w;
-                            acc = fmaf(w, v[k], acc);
-                        }
-                        mx = top;
+                    if (whole) {
+                        c.put_row(h, Z, inv, static_cast<T*>(p.out) + (qh0 + head) * D);
+                    } else {
+                        c.put_row(h, Z, inv, p.partial + (record * p.heads + head) * D);
+                        if (lane < 4) p.lse[record * p.heads + head] = L == 0.f ? -INFINITY : c.m[h] + log2f(L);
                     }
-                    static_cast<T*>(p.out)[(qh0 + head) * D + d] =
-                        Elem<T>::from_float(sum == 0.f ? 0.f : acc / sum);
                 }
             }
+            if (!whole) {
+                const int c0 = owner(unit_lo), c1 = owner(unit_lo + seg.tiles - 1);
+                __syncwarp();  // the ticket's release covers the stores of the warp before it
+                unsigned int old = 0;
+                if (lane == 0)
+                    asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;"
+                                 : "=r"(old) : "l"(p.tickets + unit), "r"((unsigned int)(c1 - c0)) : "memory");
+                if (__shfl_sync(0xffffffffu, old, 0) == (unsigned int)(c1 - c0))
+                    join_partials<T, D>(p, unit + c0, c1 - c0 + 1, heads, qh0, lane, 32);
+            }
+        } else {
+            // ---- join the warps: common maximum, then sums in the order of the warps
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float L = column_sum(c.l[h]), Z = column_sum(c.z[h]);
+                if (lane < 4) {
+                    stats[warp * 8 + 2 * c.q4 + h] = c.m[h];
+                    stats[(W + warp) * 8 + 2 * c.q4 + h] = L;
+                    stats[(2 * W + warp) * 8 + 2 * c.q4 + h] = Z;
+                }
+            }
+            __syncthreads();
+            auto joined_max = [&](int head) {
+                float mx = stats[head];
+#pragma unroll
+                for (int w = 1; w < W; ++w) mx = fmaxf(mx, stats[w * 8 + head]);
+                return mx;
+            };
+            float f[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                f[h] = c.m[h] == -INFINITY ? 0.f : exp2_fast(c.m[h] - joined_max(2 * c.q4 + h));
+            for (int h0 = 0; h0 < heads; h0 += 4) {  // four heads at a time
+                // warp w sums heads h0 + w, h0 + w + W, ...
+                constexpr int PER = (4 + W - 1) / W;
+                float inv[PER], zj[PER];
+#pragma unroll
+                for (int r = 0; r < PER; ++r) {
+                    const int head = h0 + warp + r * W;
+                    inv[r] = zj[r] = 0.f;
+                    if (head < min(heads, h0 + 4)) {
+                        const float mx = joined_max(head);
+                        float L = 0.f, Z = 0.f;
+#pragma unroll
+                        for (int w = 0; w < W; ++w) {
+                            const float mw = stats[w * 8 + head];
+                            const float fw = mw == -INFINITY ? 0.f : exp2_fast(mw - mx);
+                            L = fmaf(stats[(W + w) * 8 + head], fw, L);
+                            Z = fmaf(stats[(2 * W + w) * 8 + head], fw, Z);
+                        }
+                        inv[r] = L == 0.f ? 0.f : 1.f / L;
+                        zj[r] = Z;
+                        if (!whole && lane == 0)
+                            p.lse[record * p.heads + head] = L == 0.f ? -INFINITY : mx + log2f(L);
+                    }
+                }
+                for (int u = 0; u < Consumer::kPieces; ++u) {
+                    if (u || h0) __syncthreads();
+                    if (c.q4 >> 1 == h0 >> 2) c.put_piece(u, f, piece + warp * 128);
+                    __syncthreads();
+#pragma unroll
+                    for (int r = 0; r < PER; ++r) {
+                        const int head = h0 + warp + r * W;
+                        if (head < min(heads, h0 + 4)) {
+                            float sum = zj[r];
+#pragma unroll
+                            for (int w = 0; w < W; ++w) sum += piece[w * 128 + (head - h0) * 32 + lane];
+                            const int d = Consumer::dim_of(u, lane);
+                            if (whole)
+                                static_cast<T*>(p.out)[(qh0 + head) * D + d] = Elem<T>::from_float(sum * inv[r]);
+                            else
+                                p.partial[(record * p.heads + head) * D + d] = sum * inv[r];
+                        }
+                    }
+                }
+            }
+            if (!whole) {
+                // ---- the CTA that takes the unit's last ticket joins its partials
+                const int c0 = owner(unit_lo), c1 = owner(unit_lo + seg.tiles - 1);
+                __syncthreads();  // the ticket's release covers the stores of the CTA before it
+                if (tid == 0) {
+                    unsigned int old;
+                    asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;"
+                                 : "=r"(old) : "l"(p.tickets + unit), "r"((unsigned int)(c1 - c0)) : "memory");
+                    last_ticket = old == (unsigned int)(c1 - c0);
+                }
+                __syncthreads();
+                if (last_ticket) join_partials<T, D>(p, unit + c0, c1 - c0 + 1, heads, qh0, tid, W * 32);
+            }
+            __syncthreads();  // stats, piece (the consumers' scratch) and last_ticket are free again
         }
-        __syncthreads();  // stats, piece and last_ticket are free again
-        advance(seg, (int)(hi - lo));
-        lo = hi;
+        const int n = end - done;
+        done = end;
+        if (done < run) advance(seg, n);
     }
 }
 
 // ------------------------------------------------------------------ host side
 struct PageDecodePlan {
     int grid, smem, chunks, heads;
-    int64_t units, ws_lse, ws_partial, ws_bytes;
+    int64_t units, ws_lse, ws_bytes;
 };
 
 // Shapes and the device only: graph-static.
 template <typename Consumer, bool INT4>
-static bool page_decode_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int sms, PageDecodePlan* plan) {
+static void page_decode_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int sms, PageDecodePlan* plan) {
     using Shape = PageShape<Consumer, INT4>;
-    const int64_t smem = Shape::kFixed + (B + 1) * 4;
-    if (smem > 227 * 1024 - 1024) return false;
-    const int per_sm = D <= 128 && 2 * (smem + 2048) <= 227 * 1024 ? 2 : 1;
+    constexpr int smem = Shape::kBytes;
+    static_assert(smem <= 227 * 1024 - 512, "does not fit shared memory");
+    // 228 KB an SM, of which each block takes 1 KB and its static arrays besides
+    const int per_sm = D <= 128 && 2 * (smem + 1024 + 256) <= 228 * 1024 ? 2 : 1;
     const int64_t group = Hq / Hkv;
     plan->chunks = (int)((group + 7) / 8);
     plan->heads = (int)(group < 8 ? group : 8);
     plan->units = B * Hkv * plan->chunks;
     plan->grid = sms * per_sm;
-    plan->smem = (int)smem;
-    const int64_t records = plan->units + plan->grid;
+    plan->smem = smem;
+    const int64_t records = plan->units + (int64_t)plan->grid * Shape::kWarps;
     plan->ws_lse = (records * plan->heads * 4 + 255) / 256 * 256;
-    plan->ws_partial = 0;
     plan->ws_bytes = plan->ws_lse + records * plan->heads * D * 4;
-    return true;
 }
 
 }  // namespace minikv

@@ -145,18 +145,18 @@ template <typename F> auto with_consumer(bool int4, int dtype, int64_t dim, F f)
     });
 }
 
-bool decode_plan(bool int4, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int dtype,
+void decode_plan(bool int4, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int dtype,
                  PageDecodePlan* plan) {
     const int sms = sm_count();
-    return with_consumer(int4, dtype, dim, [&](auto c, auto, auto, auto i) {
-        return page_decode_plan<typename decltype(c)::type, decltype(i)::value>(batch, q_heads, kv_heads, dim, sms,
-                                                                               plan);
+    with_consumer(int4, dtype, dim, [&](auto c, auto, auto, auto i) {
+        page_decode_plan<typename decltype(c)::type, decltype(i)::value>(batch, q_heads, kv_heads, dim, sms, plan);
+        return 0;
     });
 }
 
-template <typename T, int D, typename Consumer, bool INT4, bool SELECTED>
+template <typename T, int D, typename Consumer, bool INT4, bool SELECTED, bool ALIGNED>
 cudaError_t launch_page_decode(const PageDecodeParams& p, const PageDecodePlan& plan, cudaStream_t stream) {
-    auto kernel = page_decode_kernel<T, D, Consumer, INT4, SELECTED>;
+    auto kernel = page_decode_kernel<T, D, Consumer, INT4, SELECTED, ALIGNED>;
     static int configured[64] = {0};
     const cudaError_t err = ensure_smem(kernel, plan.smem, configured);
     if (err != cudaSuccess) return err;
@@ -176,8 +176,7 @@ int run_page_decode(bool int4, const void* query, const void* key_cache, const v
     PAGES_REQUIRE(aligned16(query) && aligned16(key_cache) && aligned16(value_cache) && aligned16(out), MINIKV_EINVAL,
                   "query, caches and output must be 16-byte aligned");
     PageDecodePlan plan;
-    if (!decode_plan(int4, batch, q_heads, kv_heads, dim, dtype, &plan))
-        return minikv_set_error(MINIKV_EUNSUPPORTED, "decode shape does not fit shared memory (batch too large?)");
+    decode_plan(int4, batch, q_heads, kv_heads, dim, dtype, &plan);
     PAGES_REQUIRE(tickets && workspace && workspace_bytes >= plan.ws_bytes && aligned16(workspace), MINIKV_EINVAL,
                   "decode workspace too small or misaligned");
     PageDecodeParams p{};
@@ -219,9 +218,13 @@ int run_page_decode(bool int4, const void* query, const void* key_cache, const v
         constexpr int D = decltype(d)::value;
         constexpr bool I = decltype(i)::value;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const bool aligned = block_size % 16 == 0;
         if constexpr (I)
-            if (selected == nullptr) return launch_page_decode<T, D, C, I, false>(p, plan, s);
-        return launch_page_decode<T, D, C, I, true>(p, plan, s);
+            if (selected == nullptr)
+                return aligned ? launch_page_decode<T, D, C, I, false, true>(p, plan, s)
+                               : launch_page_decode<T, D, C, I, false, false>(p, plan, s);
+        return aligned ? launch_page_decode<T, D, C, I, true, true>(p, plan, s)
+                       : launch_page_decode<T, D, C, I, true, false>(p, plan, s);
     });
     if (err != cudaSuccess) return cuda_fail(err, "page decode launch");
     return MINIKV_OK;
@@ -301,10 +304,7 @@ int64_t minikv_paged_decode_int4_workspace_bytes(int64_t batch, int64_t q_heads,
     if (check_decode(batch, q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, 1, false, dtype))
         return -1;
     PageDecodePlan plan;
-    if (!decode_plan(true, batch, q_heads, kv_heads, head_dim, dtype, &plan)) {
-        minikv_set_error(MINIKV_EUNSUPPORTED, "decode shape does not fit shared memory (batch too large?)");
-        return -1;
-    }
+    decode_plan(true, batch, q_heads, kv_heads, head_dim, dtype, &plan);
     return plan.ws_bytes;
 }
 
@@ -504,10 +504,7 @@ int64_t minikv_paged_decode_selected_workspace_bytes(int64_t batch, int64_t q_he
     if (check_decode(batch, q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, 1, false, dtype))
         return -1;
     PageDecodePlan plan;
-    if (!decode_plan(false, batch, q_heads, kv_heads, head_dim, dtype, &plan)) {
-        minikv_set_error(MINIKV_EUNSUPPORTED, "decode shape does not fit shared memory (batch too large?)");
-        return -1;
-    }
+    decode_plan(false, batch, q_heads, kv_heads, head_dim, dtype, &plan);
     return plan.ws_bytes;
 }
 

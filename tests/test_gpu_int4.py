@@ -155,6 +155,23 @@ def test_decode_splits(cuda_device, lens):
     decode(np.random.default_rng(len(lens)), torch.bfloat16, lens, 16, 8, 64, 16)
 
 
+def test_decode_of_more_requests_than_threads(cuda_device):
+    """700 requests, some of them without a token, on few pages."""
+    gen = np.random.default_rng(17)
+    kp, vp = make_pool(gen, 30, 16, 2, 32), make_pool(gen, 30, 16, 2, 32)
+    lens = torch.from_numpy(gen.integers(0, 90, size=700).astype(np.int64))
+    lens[5:9] = 0
+    lens[690:] = torch.tensor([0, 0, 1, 89, 1 << 40, -1, 33, 0, 0, 0])
+    table = torch.from_numpy(gen.integers(0, 30, size=(700, 6)).astype(np.int64))
+    query = randn(gen, 700, 4, 32).to(torch.float16)
+    keys, vals = int4_kv.values(kp, 16, 32), int4_kv.values(vp, 16, 32)
+    expected = int4_kv.paged_decode(query, keys, vals, table, lens, 16)
+    actual = paged_attention_int4(query.cuda(), torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(), table.cuda(),
+                                  lens.cuda(), 16, validate=False)
+    assert_near(actual, expected, query, keys, vals, torch.float16, False)
+    assert not actual[lens <= 0].any()
+
+
 @pytest.mark.parametrize("scale,q_scale", [(2.0 ** -12, 1.0), (3000.0, 2.0 ** -8), (1.0, 2.0 ** -40), (2.0 ** -9, 2.0 ** 30)])
 def test_decode_extreme_scales(cuda_device, scale, q_scale):
     decode(np.random.default_rng(9), torch.bfloat16, (40, 700), 8, 2, 64, 16, scale=scale, q_scale=q_scale)

@@ -148,9 +148,6 @@ def test_c_entry_points_refuse():
         refused(entry(ctypes.c_void_p(8), *decode[1:], 2, 8, 4, 64, 10, 16, 4, 2, _lib.BF16, None), "aligned")
         refused(entry(*decode[:9], 16, 2, 8, 4, 64, 10, 16, 4, 2, _lib.BF16, None), "workspace")
     refused(lib.minikv_paged_decode_selected(*decode[:5], None, *decode[6:], 2, 8, 4, 64, 10, 16, 4, 2, _lib.BF16, None), "null")
-    big = 1 << 20  # a batch whose tile counts do not fit shared memory
-    assert lib.minikv_paged_decode_int4(*decode, big, 8, 4, 64, 10, 16, 4, 2, _lib.BF16, None) == _lib.EUNSUPPORTED
-    assert lib.minikv_paged_decode_int4_workspace_bytes(big, 8, 4, 64, 10, 16, 4, _lib.BF16) == -1
     assert lib.minikv_paged_decode_int4_workspace_bytes(2, 8, 4, 64, 10, 16, 4, _lib.BF16) > 0
     assert lib.minikv_paged_decode_selected_workspace_bytes(2, 8, 4, 80, 10, 16, 4, _lib.BF16) == -1
     refused(lib.minikv_kv_scatter_slots_int4(p, p, p, p, p, 3, 8, 16, 2, 64, 127, 128, _lib.BF16, None), "stride")
