@@ -19,6 +19,8 @@
 // of a 16-bit block of 16 tokens (K and V: 64 D bytes).
 #pragma once
 
+#include <string.h>
+
 #include "common.cuh"
 #include "int4_pool.cuh"
 
@@ -78,6 +80,86 @@ template <bool UP> __device__ __forceinline__ int bound_code(float x, float top,
     return min(127, max(-127, c));
 }
 
+// Running elementwise maximum and minimum of a lane's E elements, and whether any was NaN or infinite.
+// 16-bit pools keep them packed, two elements an operation.
+template <typename T, int E> struct Extremes {
+    static constexpr bool PACKED = E % 2 == 0 && (std::is_same<T, __half>::value || std::is_same<T, __nv_bfloat16>::value);
+    using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    float hi[E], lo[E];
+    uint32_t phi[E / 2 + 1], plo[E / 2 + 1], bad[E / 2 + 1];
+    float odd;
+
+    __device__ __forceinline__ void start() {
+        if constexpr (PACKED) {
+            // the type's infinities: above and below every finite value
+            constexpr uint32_t inf = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) {
+                phi[i] = inf | 0x80008000u;
+                plo[i] = inf;
+                bad[i] = 0u;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                hi[i] = -INFINITY;
+                lo[i] = INFINITY;
+            }
+            odd = 0.f;
+        }
+    }
+    __device__ __forceinline__ void add(const uint32_t* w) {  // packed
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+            const Pair x = *reinterpret_cast<const Pair*>(&w[i]);
+            Pair h = *reinterpret_cast<Pair*>(&phi[i]), l = *reinterpret_cast<Pair*>(&plo[i]);
+            Pair z = *reinterpret_cast<Pair*>(&bad[i]);
+            const uint32_t zero = 0u;
+            h = __hmax2(h, x);
+            l = __hmin2(l, x);
+            z = __hfma2(x, *reinterpret_cast<const Pair*>(&zero), z);  // NaN from NaN and infinities
+            phi[i] = *reinterpret_cast<uint32_t*>(&h);
+            plo[i] = *reinterpret_cast<uint32_t*>(&l);
+            bad[i] = *reinterpret_cast<uint32_t*>(&z);
+        }
+    }
+    __device__ __forceinline__ void add(const float* f) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            hi[i] = fmaxf(hi[i], f[i]);
+            lo[i] = fminf(lo[i], f[i]);
+            odd = fmaf(f[i], 0.f, odd);
+        }
+    }
+    __device__ __forceinline__ void add_careful(const float* f) {  // NaN as 0, infinities as the largest
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float x = isnan(f[i]) ? 0.f : fminf(fmaxf(f[i], -kLargest), kLargest);
+            hi[i] = fmaxf(hi[i], x);
+            lo[i] = fminf(lo[i], x);
+        }
+    }
+    __device__ __forceinline__ bool is_odd() const {
+        if constexpr (PACKED) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) any |= bad[i];
+            return (any & 0x7fff7fffu) != 0u;
+        } else {
+            return !(odd == 0.f);
+        }
+    }
+    __device__ __forceinline__ void finish() {
+        if constexpr (PACKED) {
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) {
+                Elem<T>::unpack(phi[i], hi + 2 * i);
+                Elem<T>::unpack(plo[i], lo + 2 * i);
+            }
+        }
+    }
+};
+
 // One warp per (request, touched block, kv head): reads the block's rows [0, written) and writes
 // its record.  Bound by the rows it reads.
 template <typename T, int D>
@@ -89,70 +171,92 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(
     griddep_launch_dependents();
     constexpr bool INT4 = std::is_same<T, Int4Tag>::value;
     constexpr int E = bounds_elems<T>(D), N = D / (32 * E);
+    using X = Extremes<T, E>;
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
     const int64_t units = requests * most_blocks * kv_heads;
     const int64_t page_bytes = int4_page_bytes(block_size, D);
     for (int64_t u = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
-        const int64_t rb = u / kv_heads;
+        const int64_t rb = (units >> 31) ? u / kv_heads : (int64_t)((uint32_t)u / (uint32_t)kv_heads);
         const int h = (int)(u - rb * kv_heads);
-        const int64_t r = rb / most_blocks;
+        const int64_t r = (units >> 31) ? rb / most_blocks : (int64_t)((uint32_t)rb / (uint32_t)most_blocks);
         const int64_t start = starts[r], len = lens[r];
-        if (start < 0 || len > width * block_size) continue;
-        const int64_t j = start / block_size + (rb - r * most_blocks);
-        if (start >= len || j * block_size >= len) continue;
+        if (start < 0 || len > width * block_size || start >= len) continue;
+        const int64_t j = (uint32_t)start / (uint32_t)block_size + (rb - r * most_blocks);
+        if (j * block_size >= len) continue;
         const int64_t page = tables[r * width + j];
         if (page < 0 || page >= num_blocks) continue;
         const int rows = (int)min((int64_t)block_size, len - j * block_size);
-        float hi[N][E], lo[N][E];
+        X x[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                hi[i][e] = -kLargest;
-                lo[i][e] = kLargest;
-            }
+        for (int i = 0; i < N; ++i) x[i].start();
         const unsigned char* page4 = keys + (page * kv_heads + h) * page_bytes;
-#pragma unroll 4
+        const T* page16 = reinterpret_cast<const T*>(keys) + (page * block_size * kv_heads + h) * (INT4 ? 0 : (int64_t)D);
+        auto values4 = [&](int t, int i, float* f) {  // of row t of a 4-bit page
+            const float2 sb = __half22float2(
+                *reinterpret_cast<const __half2*>(page4 + (int64_t)block_size * (D / 2) + t * 4));
+            const float s = fmaxf(sb.x, kInt4StepMin);
+            const int d = (i * 32 + lane) * E;
+            const unsigned char* src = page4 + (int64_t)t * (D / 2) + d / 2;
+            uint32_t word;
+            if constexpr (E == 8) word = *reinterpret_cast<const uint32_t*>(src);
+            else if constexpr (E == 4) word = *reinterpret_cast<const uint16_t*>(src);
+            else if constexpr (E == 2) word = *src;
+            else word = *src >> (4 * (d & 1));
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[e] = __fadd_rn(sb.y, __fmul_rn(s, (float)((word >> (4 * e)) & 15u)));
+        };
+        auto values = [&](int t, int i, float* f) {
+            if constexpr (INT4) values4(t, i, f);
+            else RowElems<T, E>::load(page16 + (int64_t)t * kv_heads * D, (i * 32 + lane) * E, f);
+        };
+#pragma unroll 8
         for (int t = 0; t < rows; ++t) {
-            float f[N][E];
-            if constexpr (INT4) {
-                const float2 sb = __half22float2(
-                    *reinterpret_cast<const __half2*>(page4 + (int64_t)block_size * (D / 2) + t * 4));
-                const float s = fmaxf(sb.x, kInt4StepMin);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int d = (i * 32 + lane) * E;
-                    const unsigned char* src = page4 + (int64_t)t * (D / 2) + d / 2;
-                    uint32_t word;
-                    if constexpr (E == 8) word = *reinterpret_cast<const uint32_t*>(src);
-                    else if constexpr (E == 4) word = *reinterpret_cast<const uint16_t*>(src);
-                    else if constexpr (E == 2) word = *src;
-                    else word = *src >> (4 * (d & 1));
-#pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        f[i][e] = __fadd_rn(sb.y, __fmul_rn(s, (float)((word >> (4 * e)) & 15u)));
+            for (int i = 0; i < N; ++i) {
+                if constexpr (X::PACKED) {
+                    uint32_t w[E / 2];
+                    const unsigned char* src =
+                        reinterpret_cast<const unsigned char*>(page16 + (int64_t)t * kv_heads * D + (i * 32 + lane) * E);
+                    if constexpr (E == 8) {
+                        const uint4 v = ld_global_nc(src);
+                        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+                    } else if constexpr (E == 4) {
+                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+                        w[0] = v.x; w[1] = v.y;
+                    } else {
+                        w[0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+                    }
+                    x[i].add(w);
+                } else {
+                    float f[E];
+                    values(t, i, f);
+                    x[i].add(f);
                 }
-            } else {
-                const T* row = reinterpret_cast<const T*>(keys) +
-                               ((page * block_size + t) * kv_heads + h) * (int64_t)D;
-#pragma unroll
-                for (int i = 0; i < N; ++i) RowElems<T, E>::load(row, (i * 32 + lane) * E, f[i]);
             }
+        }
 #pragma unroll
-            for (int i = 0; i < N; ++i)
+        for (int i = 0; i < N; ++i) {
+            if (x[i].is_odd()) {  // some key is NaN or infinite: again, with care
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float x = isnan(f[i][e]) ? 0.f : fminf(fmaxf(f[i][e], -kLargest), kLargest);
-                    hi[i][e] = fmaxf(hi[i][e], x);
-                    lo[i][e] = fminf(lo[i][e], x);
+                    x[i].hi[e] = -kLargest;
+                    x[i].lo[e] = kLargest;
                 }
+                for (int t = 0; t < rows; ++t) {
+                    float f[E];
+                    values(t, i, f);
+                    x[i].add_careful(f);
+                }
+            } else {
+                x[i].finish();
+            }
         }
         float top = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int e = 0; e < E; ++e) top = fmaxf(top, fmaxf(fabsf(hi[i][e]), fabsf(lo[i][e])));
+            for (int e = 0; e < E; ++e) top = fmaxf(top, fmaxf(fabsf(x[i].hi[e]), fabsf(x[i].lo[e])));
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
         const bool none = top < kBoundsNone;
@@ -161,11 +265,14 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int d = (i * 32 + lane) * E;
+            unsigned char up[E], down[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                rec[d + e] = (unsigned char)(none ? 0 : bound_code<true>(hi[i][e], top, inv));
-                rec[D + d + e] = (unsigned char)(none ? 0 : bound_code<false>(lo[i][e], top, inv));
+                up[e] = (unsigned char)(none ? 0 : bound_code<true>(x[i].hi[e], top, inv));
+                down[e] = (unsigned char)(none ? 0 : bound_code<false>(x[i].lo[e], top, inv));
             }
+            memcpy(__builtin_assume_aligned(rec + d, E), up, E);
+            memcpy(__builtin_assume_aligned(rec + D + d, E), down, E);
         }
         if (lane == 0)
             *reinterpret_cast<uint4*>(rec + 2 * D) =
@@ -173,27 +280,35 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(
     }
 }
 
-// Values of the bounds of listed blocks: lower and upper [n, kv_heads, D] (zeros for a block outside the pool).
+// Values of the bounds of listed blocks: lower and upper [n, kv_heads, D] (zeros for a block outside
+// the pool).  A thread takes four dims of a record.
 static __global__ void __launch_bounds__(256) read_bounds_kernel(
     const unsigned char* __restrict__ bounds, const int64_t* __restrict__ ids, int64_t n, int64_t num_blocks,
-    int kv_heads, int D, float* __restrict__ lower, float* __restrict__ upper) {
+    int kv_heads, int D, FastDiv quads_of, FastDiv heads_of, float* __restrict__ lower, float* __restrict__ upper) {
     griddep_wait();
     griddep_launch_dependents();
-    const int64_t quads = n * kv_heads * (D / 4);
-    for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < quads; u += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = u / (D / 4);
-        const int d = (int)(u - row * (D / 4)) * 4;
-        const int64_t id = ids[row / kv_heads];
-        float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
-        if (id >= 0 && id < num_blocks) {
-            const unsigned char* rec = bounds + (id * kv_heads + row % kv_heads) * (int64_t)(2 * D + kBoundsPad);
-            const float s = *reinterpret_cast<const float*>(rec + 2 * D);
-            const char4 a = *reinterpret_cast<const char4*>(rec + d), b = *reinterpret_cast<const char4*>(rec + D + d);
-            hi = make_float4(a.x * s, a.y * s, a.z * s, a.w * s);
-            lo = make_float4(b.x * s, b.y * s, b.z * s, b.w * s);
+    const int64_t rows = n * kv_heads;
+    // rows in pieces of 2^20, so that a piece's quads are counted in 31 bits
+    for (int64_t r0 = 0; r0 < rows; r0 += 1 << 20) {
+        const uint32_t quads = (uint32_t)min(rows - r0, (int64_t)(1 << 20)) * quads_of.d;
+#pragma unroll 2
+        for (uint32_t u = blockIdx.x * blockDim.x + threadIdx.x; u < quads; u += gridDim.x * blockDim.x) {
+            const uint32_t in = quads_of(u);
+            const int d = (int)(u - in * quads_of.d) * 4;
+            const int64_t row = r0 + in;
+            const int64_t at = (rows >> 31) ? row / kv_heads : (int64_t)heads_of((uint32_t)row);
+            const int64_t id = ids[at];
+            float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+            if (id >= 0 && id < num_blocks) {
+                const unsigned char* rec = bounds + (id * kv_heads + (row - at * kv_heads)) * (int64_t)(2 * D + kBoundsPad);
+                const float s = *reinterpret_cast<const float*>(rec + 2 * D);
+                const char4 a = *reinterpret_cast<const char4*>(rec + d), b = *reinterpret_cast<const char4*>(rec + D + d);
+                hi = make_float4(a.x * s, a.y * s, a.z * s, a.w * s);
+                lo = make_float4(b.x * s, b.y * s, b.z * s, b.w * s);
+            }
+            *reinterpret_cast<float4*>(lower + row * D + d) = lo;
+            *reinterpret_cast<float4*>(upper + row * D + d) = hi;
         }
-        *reinterpret_cast<float4*>(lower + row * D + d) = lo;
-        *reinterpret_cast<float4*>(upper + row * D + d) = hi;
     }
 }
 
@@ -206,8 +321,8 @@ __device__ __forceinline__ uint32_t score_key(float score) {
     return min(0xfffffffeu, max(1u, k));
 }
 
-constexpr int kScoreHeads = 8;    // kv heads a CTA scores
-constexpr int kScoreBlocks = 64;  // blocks a CTA scores
+constexpr int kScoreHeads = 8;   // kv heads a CTA scores
+constexpr int kScoreSpan = 512;  // blocks a CTA scores at most
 
 struct SelectParams {
     const void* q;
@@ -218,6 +333,7 @@ struct SelectParams {
     int64_t* selected;  // [batch, kv_heads, take]
     int64_t width, num_blocks;
     int q_heads, kv_heads, group, block_size, take, sink, recent;
+    int span;  // blocks a CTA scores
 };
 
 __device__ __forceinline__ int blocks_of(const SelectParams& p, int64_t b) {
@@ -225,24 +341,27 @@ __device__ __forceinline__ int blocks_of(const SelectParams& p, int64_t b) {
     return len > 0 && len <= p.width * p.block_size ? (int)((len + p.block_size - 1) / p.block_size) : 0;
 }
 
-// Scores of kScoreBlocks blocks of one request for up to kScoreHeads kv heads.  Bound by the
-// records' bytes.  16 bytes of codes a lane: int4_row_lanes(D) lanes a head.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) score_blocks_kernel(const SelectParams p) {
+// Scores of p.span blocks of one request for up to kScoreHeads kv heads.  Bound by the
+// records' bytes.  16 bytes of codes a lane: int4_row_lanes(D) lanes a head.  The spans are as long
+// as fills the device once (a CTA first makes the query's codes, 3 us), and a span's keys go out
+// head by head from shared memory.
+template <typename T, int D, bool FULL>  // FULL: eight heads in every group
+__global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) score_blocks_kernel(const SelectParams p) {
     constexpr int LPH = int4_row_lanes(D);        // lanes a head (2 D / 16 of them active)
     constexpr int HPW = 32 / LPH;                 // heads a warp scores at once
-    constexpr int PASSES = kScoreHeads / HPW > 0 ? kScoreHeads / HPW : 1;
+    constexpr int PASSES = kScoreHeads / HPW;
     constexpr int REC = 2 * D + kBoundsPad;
     __shared__ float sums[kScoreHeads][2 * D];
     __shared__ int tops[kScoreHeads];
     __shared__ __align__(16) signed char codes[kScoreHeads][2 * D];
+    __shared__ uint32_t found[kScoreHeads][kScoreSpan];
     griddep_wait();
     griddep_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int64_t chunks = (p.width + kScoreBlocks - 1) / kScoreBlocks;
+    const int64_t chunks = (p.width + p.span - 1) / p.span;
     const int64_t b = blockIdx.x / chunks;
     const int n = blocks_of(p, b);
-    const int first = (int)(blockIdx.x - b * chunks) * kScoreBlocks;
+    const int first = (int)(blockIdx.x - b * chunks) * p.span;
     if (first >= n || n <= p.take) return;  // a request with no more blocks than are taken needs no scores
     const int h0 = blockIdx.y * kScoreHeads, nh = min(kScoreHeads, p.kv_heads - h0);
     // ---- the query's codes
@@ -262,7 +381,9 @@ __global__ void __launch_bounds__(256) score_blocks_kernel(const SelectParams p)
         neg = fmaxf(neg, -kLargest);
         sums[h][d] = pos;
         sums[h][D + d] = neg;
-        atomicMax(&tops[h], __float_as_int(fmaxf(pos, -neg)));  // non-negative floats order as their bits
+        // non-negative floats order as their bits
+        const int top = __reduce_max_sync(__activemask(), __float_as_int(fmaxf(pos, -neg)));
+        if (lane == 0) atomicMax(&tops[h], top);  // a warp's 32 dims are of one head
     }
     __syncthreads();
     for (int x = tid; x < kScoreHeads * 2 * D; x += 256) {
@@ -281,44 +402,63 @@ __global__ void __launch_bounds__(256) score_blocks_kernel(const SelectParams p)
 #pragma unroll
     for (int i = 0; i < PASSES; ++i)
         qc[i] = active ? *reinterpret_cast<const int4*>(&codes[i * HPW + part][sub * 16]) : make_int4(0, 0, 0, 0);
-    // ---- blocks: 8 warps, one block each at a time
-    const int last = min(n, first + kScoreBlocks);
-    const int64_t* table = p.tables + b * p.width;
+    // ---- blocks: warp w takes blocks w, w + 8, ... of the span, AHEAD of them in flight; lane x looks
+    // up the page of the warp's next x-th block for 32 of them at once
+    constexpr int AHEAD = D <= 128 ? 4 : 2;
+    const int last = min(n, first + p.span), mine = (last - first - warp + 7) / 8;
+    const int64_t* table = p.tables + b * p.width + first + warp;
     const int recent_from = n - p.recent;
-#pragma unroll 2
-    for (int j = first + warp; j < last; j += 8) {
-        const int64_t page = table[j];
-        const bool ok = page >= 0 && page < p.num_blocks;
-        const unsigned char* rec = p.bounds + ((ok ? page : 0) * p.kv_heads + h0) * (int64_t)REC;
-        int4 v[PASSES];
-        float scale[PASSES];
+    const int64_t stride = p.kv_heads * (int64_t)REC;
+    const unsigned char* lane_at = p.bounds + (int64_t)(h0 + part) * REC + (active ? sub * 16 : 0);
+    const int to_scale = 2 * D - (active ? sub * 16 : 0);
+    int64_t page = 0;
+    for (int k0 = 0; k0 < mine; k0 += AHEAD) {
+        if (k0 % 32 == 0) {
+            const int k = k0 + lane;
+            page = k < mine ? table[8 * k] : -1;
+            if (page >= p.num_blocks) page = -1;
+        }
+        int4 v[AHEAD][PASSES];
+        float scale[AHEAD][PASSES];
+        bool ok[AHEAD];
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            const int h = min(i * HPW + part, nh - 1);
-            v[i] = make_int4(0, 0, 0, 0);
-            if (active) {
-                const uint4 w = ld_global_nc(rec + (int64_t)h * REC + sub * 16);
-                v[i] = make_int4((int)w.x, (int)w.y, (int)w.z, (int)w.w);
+        for (int a = 0; a < AHEAD; ++a) {
+            const int64_t id = __shfl_sync(0xffffffffu, page, (k0 + a) % 32);
+            ok[a] = id >= 0;
+            const unsigned char* rec = lane_at + (ok[a] ? id : 0) * stride;
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                // a group of fewer heads reads its first again
+                const unsigned char* at = rec + (FULL || i * HPW + part < nh ? i * HPW * REC : -part * REC);
+                const uint4 w = ld_global_nc(at);
+                v[a][i] = make_int4((int)w.x, (int)w.y, (int)w.z, (int)w.w);
+                scale[a][i] = __ldg(reinterpret_cast<const float*>(at + to_scale));
             }
-            scale[i] = *reinterpret_cast<const float*>(rec + (int64_t)h * REC + 2 * D);
         }
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-            int dot = __dp4a(v[i].x, qc[i].x, 0);
-            dot = __dp4a(v[i].y, qc[i].y, dot);
-            dot = __dp4a(v[i].z, qc[i].z, dot);
-            dot = __dp4a(v[i].w, qc[i].w, dot);
+        for (int a = 0; a < AHEAD; ++a) {
+            const int j = first + warp + 8 * (k0 + a);
+            const bool forced = j < p.sink || j >= recent_from;
 #pragma unroll
-            for (int m = LPH / 2; m > 0; m >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, m);
-            const int h = i * HPW + part;
-            if (sub == 0 && h < nh) {
-                const float s = __fmul_rn((float)dot, scale[i]);
-                uint32_t key = isnan(s) ? 1u : score_key(s);
-                if (j < p.sink || j >= recent_from) key = 0xffffffffu;
-                p.keys[(b * p.kv_heads + h0 + h) * p.width + j] = ok ? key : 0u;
+            for (int i = 0; i < PASSES; ++i) {
+                int dot = __dp4a(v[a][i].x, qc[i].x, 0);
+                dot = __dp4a(v[a][i].y, qc[i].y, dot);
+                dot = __dp4a(v[a][i].z, qc[i].z, dot);
+                dot = __dp4a(v[a][i].w, qc[i].w, dot);
+#pragma unroll
+                for (int m = LPH / 2; m > 0; m >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, m);
+                if (sub == 0 && k0 + a < mine) {
+                    const float s = __fmul_rn((float)dot, scale[a][i]);
+                    const uint32_t key = forced ? 0xffffffffu : isnan(s) ? 1u : score_key(s);
+                    found[i * HPW + part][j - first] = ok[a] ? key : 0u;
+                }
             }
         }
     }
+    __syncthreads();
+    for (int h = 0; h < nh; ++h)
+        for (int x = tid; x < last - first; x += 256)
+            p.keys[(b * p.kv_heads + h0 + h) * p.width + first + x] = found[h][x];
 }
 
 // ------------------------------------------------------------------ selection
@@ -328,6 +468,111 @@ __global__ void __launch_bounds__(256) score_blocks_kernel(const SelectParams p)
 // selected block its place.  Keys are held in shared memory when they fit.
 constexpr int kSelectThreads = 512;
 constexpr int kSelectHeld = 24576;  // keys in shared memory (96 KB)
+
+// Sum over the CTA, in one barrier: `turn` alternates between two sets of warp sums.
+__device__ __forceinline__ int block_sum(int x, int (*sums)[32], int turn) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    x = __reduce_add_sync(0xffffffffu, x);
+    if (lane == 0) sums[turn & 1][threadIdx.x >> 5] = x;
+    __syncthreads();
+    return __reduce_add_sync(0xffffffffu, lane < warps ? sums[turn & 1][lane] : 0);
+}
+
+// Requests of up to 4096 blocks: a thread holds KEYS consecutive keys in registers, and the
+// take-th largest is found bit by bit, a count and a barrier each, until a value is met that exactly
+// `take` keys reach (a score's 32 bits rarely tie).
+template <int KEYS>
+__global__ void __launch_bounds__(512) select_few_kernel(const SelectParams p) {
+    __shared__ int counts[2][32];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    const int64_t b = blockIdx.x / p.kv_heads;
+    const int n = blocks_of(p, b);
+    int64_t* out = p.selected + (int64_t)blockIdx.x * p.take;
+    const bool all = n <= p.take;
+    uint32_t key[KEYS];
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+        const int at = tid * KEYS + i;
+        key[i] = 0;
+        if (at < n) {
+            if (all) {
+                const int64_t page = p.tables[b * p.width + at];
+                key[i] = page >= 0 && page < p.num_blocks ? 0xffffffffu : 0u;
+            } else {
+                key[i] = __ldcg(p.keys + (int64_t)blockIdx.x * p.width + at);
+            }
+        }
+    }
+    // the largest value that `take` keys reach: 0 where fewer have a page
+    uint32_t threshold = 0;
+    int above = 0;  // keys over it
+    int turn = 0;
+    if (!all) {
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t probe = threshold | (1u << bit);
+            int count = 0;
+            if constexpr (KEYS == 1) {
+                count = __syncthreads_count(key[0] >= probe);
+            } else {
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) count += key[i] >= probe;
+                count = block_sum(count, counts, turn++);
+            }
+            if (count >= p.take) threshold = probe;
+            if (count == p.take) break;  // exactly the keys from here on
+        }
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) count += key[i] > threshold;
+        above = block_sum(count, counts, turn++);
+    }
+    __syncthreads();
+    const int ties = all ? 0 : p.take - above;
+    // places, in the order of the blocks
+    int more = 0, equal = 0;
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+        more += key[i] > threshold;
+        equal += key[i] == threshold && key[i] != 0;
+    }
+    int im = more, ie = equal;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int vm = __shfl_up_sync(0xffffffffu, im, off), ve = __shfl_up_sync(0xffffffffu, ie, off);
+        if (lane >= off) {
+            im += vm;
+            ie += ve;
+        }
+    }
+    if (lane == 31) {
+        counts[0][warp] = im;
+        counts[1][warp] = ie;
+    }
+    __syncthreads();
+    int wm = lane < warps ? counts[0][lane] : 0, we = lane < warps ? counts[1][lane] : 0;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int vm = __shfl_up_sync(0xffffffffu, wm, off), ve = __shfl_up_sync(0xffffffffu, we, off);
+        if (lane >= off) {
+            wm += vm;
+            we += ve;
+        }
+    }
+    const int all_more = __shfl_sync(0xffffffffu, wm, 31), all_equal = __shfl_sync(0xffffffffu, we, 31);
+    const int before_m = __shfl_sync(0xffffffffu, wm, max(0, warp - 1)), before_e = __shfl_sync(0xffffffffu, we, max(0, warp - 1));
+    more = im - more + (warp ? before_m : 0);
+    equal = ie - equal + (warp ? before_e : 0);
+    int place = more + min(equal, ties);
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+        const bool tie = key[i] == threshold && key[i] != 0;
+        if (key[i] > threshold || (tie && equal < ties)) out[place++] = tid * KEYS + i;
+        equal += tie;
+    }
+    for (int i = all_more + min(all_equal, ties) + tid; i < p.take; i += blockDim.x) out[i] = -1;
+}
 
 // Exclusive prefix over the block of (a, b); total in *ta, *tb.
 __device__ __forceinline__ void block_prefix2(int& a, int& b, int* ta, int* tb, int (*scratch)[kSelectThreads / 32]) {

@@ -53,7 +53,6 @@ struct PageDecodeParams {
     int64_t page_stride;      // bytes of a page (all kv heads)
     int64_t head_stride;      // bytes from one kv head's part of a page to the next
     int64_t row_stride;       // bytes from one token's row to the next
-    int min_tiles;            // tiles a CTA takes at least
     float scale_log2;         // log2(e) / sqrt(D)
 };
 
@@ -686,7 +685,10 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 
     const int TW = alone ? 1 : W, rank = alone ? 0 : warp;  // warps of the team, and this one's place
     const int64_t team = alone ? (int64_t)blockIdx.x * W + warp : blockIdx.x;
     int64_t G = (int64_t)gridDim.x * (alone ? W : 1);  // runs
-    G = min(G, alone ? total : (total + p.min_tiles - 1) / p.min_tiles);  // every run has a tile
+    // Every run has a tile, of a CTA at least one for each warp; where that is no more than four a warp,
+    // a whole unit's, which then needs no join (8 x 513 tokens: 17.8 -> TIMING us).
+    const int least = longest <= 4 * W ? max(W, longest) : W;
+    G = min(G, alone ? total : (total + least - 1) / least);
     if (team >= G) return;
     const int64_t t0 = team * total / G;
     const int run = (int)((team + 1) * total / G - t0);  // the team's tiles; its warp r takes tiles r, r + TW, ...

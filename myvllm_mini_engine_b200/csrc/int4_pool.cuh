@@ -16,6 +16,10 @@
 // 1 KB runs at D = 128, block_size 16.
 #pragma once
 
+#include <string.h>
+
+#include <type_traits>
+
 #include "common.cuh"
 #include "row_maps.cuh"
 
@@ -25,60 +29,126 @@ __host__ __device__ constexpr int64_t int4_page_bytes(int64_t block_size, int64_
     return (block_size * (head_dim / 2 + 4) + 15) / 16 * 16;
 }
 
+// n / d for n < 2^31: a product and a shift.
+struct FastDiv {
+    uint32_t d, m, s;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t divisor) : d(divisor), s(0) {
+        while ((1ull << s) < divisor) ++s;
+        m = (uint32_t)((((1ull << s) - divisor) << 32) / divisor + 1);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
 constexpr float kInt4StepMin = 1.f / 16777216.f;  // 2^-24, the smallest fp16
 
 // Lanes that share a row in the row kernels: 8 elements a lane, a power of two.
 constexpr int int4_row_lanes(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
-// 8 consecutive elements at p as fp32.  VEC: p is 16-byte aligned.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_row8(const T* p, float* f) {
-    if constexpr (VEC) {
-        constexpr int n = 8 / Elem<T>::kPerVec;
+// 8 consecutive elements of a row, held as they came.  VEC: p is 16-byte aligned.
+template <typename T, bool VEC> struct Row8 {
+    uint4 v[8 / Elem<T>::kPerVec];
+    __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-        for (int i = 0; i < n; ++i)
-            Elem<T>::load(ld_global_nc(reinterpret_cast<const uint4*>(p) + i), f + i * Elem<T>::kPerVec);
-    } else {
+        for (int i = 0; i < 8 / Elem<T>::kPerVec; ++i) {
+            if constexpr (VEC) {
+                v[i] = ld_global_nc(reinterpret_cast<const uint4*>(p) + i);
+            } else {
+                T x[Elem<T>::kPerVec];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_float(p[i]);
+                for (int e = 0; e < Elem<T>::kPerVec; ++e) x[e] = p[i * Elem<T>::kPerVec + e];
+                memcpy(&v[i], x, 16);
+            }
+        }
     }
+    // Least and largest of the 8, and whether one is NaN, infinite or over 65504 in magnitude.
+    __device__ __forceinline__ bool extremes(const float* f, float* lo, float* hi) const {
+        bool odd;
+        if constexpr (sizeof(T) == 2) {  // two elements an operation
+            using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+            const Pair* x = reinterpret_cast<const Pair*>(v);
+            const uint32_t zero = 0u;
+            Pair l = __hmin2(__hmin2(x[0], x[1]), __hmin2(x[2], x[3])), h = __hmax2(__hmax2(x[0], x[1]), __hmax2(x[2], x[3]));
+            Pair bad = *reinterpret_cast<const Pair*>(&zero);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bad = __hfma2(x[i], *reinterpret_cast<const Pair*>(&zero), bad);
+            float a[2], b[2];
+            Elem<T>::unpack(*reinterpret_cast<uint32_t*>(&l), a);
+            Elem<T>::unpack(*reinterpret_cast<uint32_t*>(&h), b);
+            *lo = fminf(a[0], a[1]);
+            *hi = fmaxf(b[0], b[1]);
+            odd = (*reinterpret_cast<uint32_t*>(&bad) & 0x7fff7fffu) != 0u;  // NaN from NaN and infinities
+        } else {
+            float bad = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                *lo = fminf(*lo, f[i]);
+                *hi = fmaxf(*hi, f[i]);
+                bad = fmaf(f[i], 0.f, bad);
+            }
+            odd = !(bad == 0.f);
+        }
+        return odd || *lo < -65504.f || *hi > 65504.f;
+    }
+    __device__ __forceinline__ void values(float* f) const {
+#pragma unroll
+        for (int i = 0; i < 8 / Elem<T>::kPerVec; ++i) Elem<T>::load(v[i], f + i * Elem<T>::kPerVec);
+    }
+};
+
+// Code of one element by the format's own words.
+__device__ __forceinline__ uint32_t int4_code(float x, float base, float step) {
+    return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x - base, step)), 0.f), 15.f);
 }
 
 // Quantising write.  A unit is one row: (token, kv head, K or V); a group of
 // int4_row_lanes(D) lanes takes one, 8 elements a lane, so at D = 128 a warp
-// takes the K and the V row of a token's head.  Bound by the bytes of the
-// 16-bit rows it reads.
+// takes the K and the V row of a token's head.  The usual row costs an element
+// a subtraction, two products with the rounded inverse of the step (a little
+// above and a little below it, each rounded to a whole number by an addition of
+// 1.5 2^23) and an addition into the word: where the two agree, so does the true
+// quotient.  Where they differ, and for rows with NaN, infinities, magnitudes
+// above 65504 or codes to clamp, the lane divides.
 template <typename T, int D, bool VEC, typename Rows>
 __global__ void __launch_bounds__(256) int4_write_kernel(
     unsigned char* __restrict__ kc, unsigned char* __restrict__ vc, const T* __restrict__ k, const T* __restrict__ v,
-    int64_t tokens, int kv_heads, int64_t block_size, int64_t page_bytes, int64_t k_stride, int64_t v_stride,
-    Rows map) {
+    int64_t first_token, int64_t tokens, int kv_heads, FastDiv rows_of, FastDiv block_of, int64_t page_bytes,
+    int64_t k_stride, int64_t v_stride, Rows map) {
     griddep_wait();
     griddep_launch_dependents();
     constexpr int LPR = int4_row_lanes(D);
+    constexpr float kRound = 12582912.f;  // 1.5 2^23
     const int sub = threadIdx.x % LPR;
     const bool active = sub * 8 < D;
-    const int64_t units = tokens * kv_heads * 2;
-    const int64_t groups = (int64_t)gridDim.x * (blockDim.x / LPR);
-    // units of a block are consecutive; the loop bound is the same for a whole warp (the shuffles need all lanes)
-    const int64_t first = (int64_t)blockIdx.x * (blockDim.x / LPR) + threadIdx.x / LPR;
-    const int64_t warp_first = first - (threadIdx.x % 32) / LPR;
-    for (int64_t off = 0; warp_first + off < units; off += groups) {
-        const int64_t u = first + off;
+    const uint32_t units = (uint32_t)(tokens * kv_heads * 2);
+    const uint32_t groups = gridDim.x * (blockDim.x / LPR);
+    // the loop's bound is the same for a whole warp: the shuffles need all lanes
+    const uint32_t first = blockIdx.x * (blockDim.x / LPR) + threadIdx.x / LPR;
+    const uint32_t warp_first = first - (threadIdx.x % 32) / LPR;
+    for (uint32_t off = 0; warp_first + off < units; off += groups) {
+        const uint32_t u = first + off;
         const bool in = u < units;
-        const int64_t t = in ? u / (2 * kv_heads) : 0;
-        const int rest = in ? (int)(u - t * (2 * kv_heads)) : 0;
-        const int h = rest >> 1, which = rest & 1;
-        const int64_t row = in ? map(t) : -1;
+        const uint32_t t = rows_of(in ? u : 0);
+        const uint32_t rest = in ? u - t * rows_of.d : 0, h = rest >> 1;
+        const bool which = rest & 1;
+        const int64_t token = first_token + t;
+        const int64_t row = in ? map(token) : -1;
+        Row8<T, VEC> raw;
         float x[8];
         float lo = INFINITY, hi = -INFINITY;
-        if (row >= 0 && active) {
-            load_row8<T, VEC>((which ? v + t * v_stride : k + t * k_stride) + (int64_t)h * D + sub * 8, x);
+        if (active) {
+            raw.load((which ? v + token * v_stride : k + token * k_stride) + (int64_t)h * D + sub * 8);
+            raw.values(x);
+            const bool odd = raw.extremes(x, &lo, &hi);
+            if (odd) {
+                lo = INFINITY;
+                hi = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = isnan(x[i]) ? 0.f : fminf(fmaxf(x[i], -65504.f), 65504.f);
-                lo = fminf(lo, x[i]);
-                hi = fmaxf(hi, x[i]);
+                for (int i = 0; i < 8; ++i) {
+                    x[i] = isnan(x[i]) ? 0.f : fminf(fmaxf(x[i], -65504.f), 65504.f);
+                    lo = fminf(lo, x[i]);
+                    hi = fmaxf(hi, x[i]);
+                }
             }
         }
 #pragma unroll
@@ -89,24 +159,33 @@ __global__ void __launch_bounds__(256) int4_write_kernel(
         if (row < 0) continue;  // no shuffle follows in this iteration
         const __half base = __float2half_rn(lo);
         const __half step = __float2half_rn(fmaxf(__fdiv_rn(hi - lo, 15.f), kInt4StepMin));
-        const float b = __half2float(base), s = __half2float(step), inv = __fdiv_rn(1.f, s);
-        const int64_t page = row / block_size, off_in = row - page * block_size;
-        unsigned char* dst = (which ? vc : kc) + (page * kv_heads + h) * page_bytes;
+        const float b = __half2float(base), s = __half2float(step);
+        float inv;  // 1 / s within 2^-22
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+        const uint32_t page = block_of((uint32_t)row), off_in = (uint32_t)row - page * block_of.d;
+        unsigned char* dst = (which ? vc : kc) + ((int64_t)page * kv_heads + h) * page_bytes;
         if (active) {
-            uint32_t word = 0;
+            const float over = inv * (1.f + 1.f / 1048576.f), under = inv * (1.f - 1.f / 1048576.f);
+            uint32_t word = 0, differ = 0;
+            bool clamp = (lo - b) * inv < -0.49f || (hi - b) * inv > 15.49f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float d = x[i] - b;
-                const float q = d * inv;  // within 2e-6 of the quotient where that lies in 0..15
-                float c = rintf(q);
-                // next to a half: the true quotient decides.  Rare, so the division stays off the common path
-                if (fabsf(fabsf(q - c) - 0.5f) < 1e-4f) c = rintf(__fdiv_rn(d, s));
-                word |= (uint32_t)fminf(fmaxf(c, 0.f), 15.f) << (4 * i);
+                const uint32_t up = __float_as_uint(fmaf(d, over, kRound)), down = __float_as_uint(fmaf(d, under, kRound));
+                differ |= up ^ down;
+                word += up << (4 * i);  // 0x4b400000 + code, the constants taken out below
             }
-            *reinterpret_cast<uint32_t*>(dst + off_in * (D / 2) + sub * 4) = word;
+            word -= 0x3f400000u;  // 0x4b400000 (1 + 2^4 + 2^8 + ...) mod 2^32
+            if (differ != 0 || clamp) {
+                word = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) word |= int4_code(x[i], b, s) << (4 * i);
+            }
+            *reinterpret_cast<uint32_t*>(dst + (int64_t)off_in * (D / 2) + sub * 4) = word;
         }
         if (sub == 0)
-            *reinterpret_cast<__half2*>(dst + block_size * (D / 2) + off_in * 4) = __halves2half2(step, base);
+            *reinterpret_cast<__half2*>(dst + (int64_t)block_of.d * (D / 2) + (int64_t)off_in * 4) =
+                __halves2half2(step, base);
     }
 }
 
@@ -114,31 +193,34 @@ __global__ void __launch_bounds__(256) int4_write_kernel(
 template <typename T, int D>
 __global__ void __launch_bounds__(256) int4_read_kernel(
     const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc, T* __restrict__ k, T* __restrict__ v,
-    int64_t tokens, int kv_heads, int64_t block_size, int64_t page_bytes, SlotRows map) {
+    int64_t first_token, int64_t tokens, int kv_heads, FastDiv rows_of, FastDiv block_of, int64_t page_bytes,
+    SlotRows map) {
     griddep_wait();
     griddep_launch_dependents();
     constexpr int LPR = int4_row_lanes(D);
     const int sub = threadIdx.x % LPR;
     if (sub * 8 >= D) return;
-    const int64_t units = tokens * kv_heads * 2;
-    const int64_t groups = (int64_t)gridDim.x * (blockDim.x / LPR);
-    for (int64_t u = (int64_t)blockIdx.x * (blockDim.x / LPR) + threadIdx.x / LPR; u < units; u += groups) {
-        const int64_t t = u / (2 * kv_heads);
-        const int rest = (int)(u - t * (2 * kv_heads));
-        const int h = rest >> 1, which = rest & 1;
-        const int64_t row = map(t);
+    const uint32_t units = (uint32_t)(tokens * kv_heads * 2);
+    const uint32_t groups = gridDim.x * (blockDim.x / LPR);
+#pragma unroll 2
+    for (uint32_t u = blockIdx.x * (blockDim.x / LPR) + threadIdx.x / LPR; u < units; u += groups) {
+        const uint32_t t = rows_of(u);
+        const uint32_t rest = u - t * rows_of.d, h = rest >> 1;
+        const bool which = rest & 1;
+        const int64_t token = first_token + t;
+        const int64_t row = map(token);
         float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (row >= 0) {
-            const int64_t page = row / block_size, off_in = row - page * block_size;
-            const unsigned char* src = (which ? vc : kc) + (page * kv_heads + h) * page_bytes;
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(src + off_in * (D / 2) + sub * 4);
-            const float2 sb =
-                __half22float2(*reinterpret_cast<const __half2*>(src + block_size * (D / 2) + off_in * 4));
+            const uint32_t page = block_of((uint32_t)row), off_in = (uint32_t)row - page * block_of.d;
+            const unsigned char* src = (which ? vc : kc) + ((int64_t)page * kv_heads + h) * page_bytes;
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(src + (int64_t)off_in * (D / 2) + sub * 4);
+            const float2 sb = __half22float2(*reinterpret_cast<const __half2*>(
+                src + (int64_t)block_of.d * (D / 2) + (int64_t)off_in * 4));
             const float s = fmaxf(sb.x, kInt4StepMin);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(sb.y, __fmul_rn(s, (float)((word >> (4 * i)) & 15u)));
         }
-        uint4* dst = reinterpret_cast<uint4*>((which ? v : k) + (t * kv_heads + h) * D + sub * 8);
+        uint4* dst = reinterpret_cast<uint4*>((which ? v : k) + (token * kv_heads + h) * D + sub * 8);
 #pragma unroll
         for (int i = 0; i < 8 / Elem<T>::kPerVec; ++i) dst[i] = Elem<T>::store(x + i * Elem<T>::kPerVec);
     }
@@ -150,24 +232,41 @@ inline unsigned int4_grid(int64_t units, int lanes, int sms) {
     return (unsigned)(blocks < 1 ? 1 : blocks < cap ? blocks : cap);
 }
 
+// Tokens of a launch: its rows are counted in 31 bits.
+inline int64_t int4_tokens_at_once(int kv_heads) { return (1ll << 30) / kv_heads; }
+
 template <typename T, int D, typename Rows>
 static cudaError_t launch_int4_write(void* kc, void* vc, const void* k, const void* v, int64_t tokens, int kv_heads,
                                      int64_t block_size, int64_t k_stride, int64_t v_stride, bool vec, Rows map,
                                      int sms, cudaStream_t stream) {
-    return launch_chained(vec ? int4_write_kernel<T, D, true, Rows> : int4_write_kernel<T, D, false, Rows>,
-                          dim3(int4_grid(tokens * kv_heads * 2, int4_row_lanes(D), sms)), dim3(256), 0, stream,
-                          static_cast<unsigned char*>(kc), static_cast<unsigned char*>(vc), static_cast<const T*>(k),
-                          static_cast<const T*>(v), tokens, kv_heads, block_size, int4_page_bytes(block_size, D),
-                          k_stride, v_stride, map);
+    const int64_t most = int4_tokens_at_once(kv_heads) - 1;
+    cudaError_t err = cudaSuccess;
+    for (int64_t t = 0; t < tokens && err == cudaSuccess; t += most) {
+        const int64_t n = tokens - t < most ? tokens - t : most;
+        err = launch_chained(vec ? int4_write_kernel<T, D, true, Rows> : int4_write_kernel<T, D, false, Rows>,
+                             dim3(int4_grid(n * kv_heads * 2, int4_row_lanes(D), sms)), dim3(256), 0, stream,
+                             static_cast<unsigned char*>(kc), static_cast<unsigned char*>(vc),
+                             static_cast<const T*>(k), static_cast<const T*>(v), t, n, kv_heads,
+                             FastDiv((uint32_t)kv_heads * 2), FastDiv((uint32_t)block_size),
+                             int4_page_bytes(block_size, D), k_stride, v_stride, map);
+    }
+    return err;
 }
 
 template <typename T, int D>
 static cudaError_t launch_int4_read(const void* kc, const void* vc, void* k, void* v, int64_t tokens, int kv_heads,
                                     int64_t block_size, SlotRows map, int sms, cudaStream_t stream) {
-    return launch_chained(int4_read_kernel<T, D>, dim3(int4_grid(tokens * kv_heads * 2, int4_row_lanes(D), sms)),
-                          dim3(256), 0, stream, static_cast<const unsigned char*>(kc),
-                          static_cast<const unsigned char*>(vc), static_cast<T*>(k), static_cast<T*>(v), tokens,
-                          kv_heads, block_size, int4_page_bytes(block_size, D), map);
+    const int64_t most = int4_tokens_at_once(kv_heads) - 1;
+    cudaError_t err = cudaSuccess;
+    for (int64_t t = 0; t < tokens && err == cudaSuccess; t += most) {
+        const int64_t n = tokens - t < most ? tokens - t : most;
+        err = launch_chained(int4_read_kernel<T, D>, dim3(int4_grid(n * kv_heads * 2, int4_row_lanes(D), sms)),
+                             dim3(256), 0, stream, static_cast<const unsigned char*>(kc),
+                             static_cast<const unsigned char*>(vc), static_cast<T*>(k), static_cast<T*>(v), t, n,
+                             kv_heads, FastDiv((uint32_t)kv_heads * 2), FastDiv((uint32_t)block_size),
+                             int4_page_bytes(block_size, D), map);
+    }
+    return err;
 }
 
 }  // namespace minikv

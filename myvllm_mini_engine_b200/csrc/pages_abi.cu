@@ -210,7 +210,6 @@ int run_page_decode(bool int4, const void* query, const void* key_cache, const v
         p.row_stride = kv_heads * dim * 2;
         p.page_stride = block_size * p.row_stride;
     }
-    p.min_tiles = 8;
     p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)dim));
     const cudaError_t err = with_consumer(int4, dtype, dim, [&](auto c, auto t, auto d, auto i) {
         using C = typename decltype(c)::type;
@@ -418,7 +417,8 @@ int minikv_block_bounds_read(const void* bounds, const int64_t* block_ids, int64
     const int64_t grid = std::min<int64_t>((quads + 255) / 256, (int64_t)sm_count() * 8);
     const cudaError_t err = launch_chained(read_bounds_kernel, dim3((unsigned)grid), dim3(256), 0,
                                            static_cast<cudaStream_t>(stream), static_cast<const unsigned char*>(bounds),
-                                           block_ids, count, num_blocks, (int)kv_heads, (int)head_dim, lower, upper);
+                                           block_ids, count, num_blocks, (int)kv_heads, (int)head_dim,
+                                           FastDiv((uint32_t)head_dim / 4), FastDiv((uint32_t)kv_heads), lower, upper);
     if (err != cudaSuccess) return cuda_fail(err, "minikv_block_bounds_read launch");
     return MINIKV_OK;
 }
@@ -436,8 +436,7 @@ static int check_select(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_
     PAGES_REQUIRE(max_blocks > 0 && max_blocks <= 1048576 && sink >= 0 && recent >= 0 &&
                       sink + recent <= max_blocks,
                   MINIKV_EINVAL, "max_blocks must be positive and hold the sink and recent blocks");
-    const int64_t chunks = (table_width + kScoreBlocks - 1) / kScoreBlocks;
-    PAGES_REQUIRE(batch <= 2147483647 / std::max<int64_t>(kv_heads, chunks), MINIKV_EINVAL, "batch/head product too large");
+    PAGES_REQUIRE(batch <= 2147483647 / std::max<int64_t>(kv_heads, table_width), MINIKV_EINVAL, "batch/head product too large");
     return MINIKV_OK;
 }
 
@@ -477,16 +476,34 @@ int minikv_select_blocks(const void* query, const void* bounds, const int64_t* b
     p.recent = (int)recent_blocks;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err = cudaSuccess;
-    const int64_t chunks = (table_width + kScoreBlocks - 1) / kScoreBlocks;
     if (table_width > max_blocks) {  // else every request takes all of its blocks
-        const dim3 grid((unsigned)(batch * chunks), (unsigned)((kv_heads + kScoreHeads - 1) / kScoreHeads));
+        const int64_t head_groups = (kv_heads + kScoreHeads - 1) / kScoreHeads;
+        // as many spans as two CTAs a SM (their registers) hold at once, each of whole turns of 8 warps
+        const int64_t spans = std::max<int64_t>(1, 2 * sm_count() / (batch * head_groups));
+        const int64_t span = std::min<int64_t>(kScoreSpan, ((table_width + spans - 1) / spans + 7) / 8 * 8);
+        p.span = (int)span;
+        const dim3 grid((unsigned)(batch * ((table_width + span - 1) / span)), (unsigned)head_groups);
         err = with_type(dtype, [&](auto t) {
             return with_dim(head_dim, [&](auto d) {
-                return launch_chained(score_blocks_kernel<typename decltype(t)::type, decltype(d)::value>, grid,
-                                      dim3(256), 0, s, p);
+                using T = typename decltype(t)::type;
+                constexpr int D = decltype(d)::value;
+                return launch_chained(kv_heads % kScoreHeads == 0 ? score_blocks_kernel<T, D, true>
+                                                                  : score_blocks_kernel<T, D, false>,
+                                      grid, dim3(256), 0, s, p);
             });
         });
         if (err != cudaSuccess) return cuda_fail(err, "minikv_select_blocks scores");
+    }
+    if (table_width <= 4096) {
+        const int keys = table_width <= 512 ? 1 : table_width <= 1024 ? 2 : table_width <= 2048 ? 4 : 8;
+        const int threads = (int)(((table_width + keys - 1) / keys + 31) / 32 * 32);
+        const dim3 grid((unsigned)(batch * kv_heads));
+        err = keys == 1   ? launch_chained(select_few_kernel<1>, grid, dim3(threads), 0, s, p)
+              : keys == 2 ? launch_chained(select_few_kernel<2>, grid, dim3(threads), 0, s, p)
+              : keys == 4 ? launch_chained(select_few_kernel<4>, grid, dim3(threads), 0, s, p)
+                          : launch_chained(select_few_kernel<8>, grid, dim3(threads), 0, s, p);
+        if (err != cudaSuccess) return cuda_fail(err, "minikv_select_blocks launch");
+        return MINIKV_OK;
     }
     const int held = (int)std::min<int64_t>(table_width, kSelectHeld);
     static int configured[64] = {0};

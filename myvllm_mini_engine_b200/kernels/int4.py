@@ -16,8 +16,8 @@ row (one token, one kv head, K or V by itself), and read as ``base + step * code
 NaN counts as 0 and magnitudes saturate at 65504.  At head_dim 128 that is 4.25
 bits an element: a decode step streams 68 bytes where a 16-bit pool has 256.
 
-Scratch memory comes from torch's caching allocator (a captured graph gets its
-own); the decode's ticket counters are kept per stream for eager calls.
+The decode's scratch memory is kept per stream for eager calls; a captured graph
+gets its own.
 """
 
 from __future__ import annotations
@@ -44,25 +44,34 @@ def int4_page_bytes(block_size, head_dim):
 
 def _check_pools(key_cache, value_cache, block_size, head_dim, fail=ValueError):
     """Shape and dtype checks shared by the operators over a pool; the pool's ``(num_blocks, kv_heads)``."""
-    if (key_cache.ndim != 3 or value_cache.shape != key_cache.shape or key_cache.dtype != torch.uint8
-            or value_cache.dtype != torch.uint8 or not key_cache.is_contiguous() or not value_cache.is_contiguous()
-            or key_cache.numel() == 0):
+    shape = key_cache.shape
+    if (len(shape) != 3 or value_cache.shape != shape or key_cache.dtype is not torch.uint8
+            or value_cache.dtype is not torch.uint8 or not key_cache.is_contiguous()
+            or not value_cache.is_contiguous() or 0 in shape):
         raise fail("4-bit KV caches must be contiguous uint8 [pages, kv_heads, page_bytes]")
     if head_dim not in INT4_HEAD_DIMS:
         raise fail(_HEAD_DIM_MESSAGE)
     if type(block_size) is not int or block_size <= 0:
         raise fail("block size mismatch")
-    if key_cache.shape[2] != int4_page_bytes(block_size, head_dim):
+    if shape[2] != (block_size * (head_dim // 2 + 4) + 15) // 16 * 16:
         raise fail("block size mismatch: the pages are not int4_page_bytes(block_size, head_dim) long")
-    return key_cache.shape[0], key_cache.shape[1]
+    return shape[0], shape[1]
+
+
+def _device_of(tensors, fail, message):
+    """The device that all of the tensors are on."""
+    index = tensors[0].get_device()
+    for tensor in tensors:
+        if tensor.get_device() != index:
+            raise fail(message)
+    return tensors[0].device
 
 
 def _source_rows(tensor):
     """(tensor, token stride) of a ``[tokens, kv_heads, head_dim]`` source whose heads are contiguous (copied if not)."""
-    heads, dim = tensor.shape[1], tensor.shape[2]
-    if tensor.shape[0] <= 1:
-        rows = tensor.contiguous()
-        return rows, heads * dim
+    _, heads, dim = tensor.shape
+    if tensor.is_contiguous():
+        return tensor, heads * dim
     if tensor.stride(2) == 1 and (heads == 1 or tensor.stride(1) == dim) and tensor.stride(0) >= heads * dim:
         return tensor, tensor.stride(0)
     return tensor.contiguous(), heads * dim
@@ -82,19 +91,21 @@ def write_kv_cache_slots_int4(key_cache, value_cache, slot_mapping, key, value, 
     of ``write_kv_cache_slots`` (data.py:109-119).
     """
     _backend(backend)
-    if key.ndim != 3 or key.shape != value.shape:
+    shape = key.shape
+    if len(shape) != 3 or value.shape != shape:
         raise ValueError("packed key/value must be [tokens, kv_heads, head_dim] matching the cache")
-    num_blocks, kv_heads = _check_pools(key_cache, value_cache, block_size, key.shape[2])
-    if key.shape[1] != kv_heads:
+    tokens, heads, dim = shape
+    num_blocks, kv_heads = _check_pools(key_cache, value_cache, block_size, dim)
+    if heads != kv_heads:
         raise ValueError("packed key/value must be [tokens, kv_heads, head_dim] matching the cache")
-    if key.dtype not in _lib.DTYPE_CODES or value.dtype != key.dtype:
+    code = _lib.DTYPE_CODES.get(key.dtype)
+    if code is None or value.dtype is not key.dtype:
         raise ValueError("packed KV requires FP32/FP16/BF16")
-    if (slot_mapping.ndim != 1 or slot_mapping.shape[0] != key.shape[0]
-            or slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous()):
+    if (slot_mapping.shape != (tokens,) or slot_mapping.dtype is not torch.int64
+            or not slot_mapping.is_contiguous()):
         raise ValueError("slot_mapping must be contiguous int64 [tokens]")
-    device = key_cache.device
-    if not (value_cache.device == slot_mapping.device == key.device == value.device == device):
-        raise ValueError("packed KV tensors and slots must share the cache device")
+    device = _device_of((key_cache, value_cache, slot_mapping, key, value), ValueError,
+                        "packed KV tensors and slots must share the cache device")
     if validate:
         slots = slot_mapping.tolist()
         if any(slot < 0 or slot >= num_blocks * block_size for slot in slots):
@@ -105,7 +116,6 @@ def write_kv_cache_slots_int4(key_cache, value_cache, slot_mapping, key, value, 
             raise ValueError("KV destinations and source tensors must not overlap")
     if device.type != "cuda":
         raise ValueError("CUDA packed KV writes require CUDA tensors")
-    tokens = key.shape[0]
     if tokens == 0:
         return
     key, key_stride = _source_rows(key)
@@ -114,9 +124,9 @@ def write_kv_cache_slots_int4(key_cache, value_cache, slot_mapping, key, value, 
     with _lib.on_device(device):
         status = lib.minikv_kv_scatter_slots_int4(
             key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(), key.data_ptr(), value.data_ptr(),
-            tokens, num_blocks, block_size, kv_heads, key.shape[2], key_stride, value_stride,
-            _lib.DTYPE_CODES[key.dtype], _lib.stream_of(device))
-    _lib.check(status, "write_kv_cache_slots_int4")
+            tokens, num_blocks, block_size, kv_heads, dim, key_stride, value_stride, code, _lib.stream_of(device))
+    if status:
+        _lib.check(status, "write_kv_cache_slots_int4")
 
 
 def write_kv_cache_batch_int4(key_cache, value_cache, block_tables, token_offsets, key, value, block_size, *,
@@ -141,9 +151,8 @@ def write_kv_cache_batch_int4(key_cache, value_cache, block_tables, token_offset
             or token_offsets.dtype != torch.int64 or not block_tables.is_contiguous()
             or not token_offsets.is_contiguous()):
         raise ValueError("batch metadata must be contiguous int64 [batch, pages] and [batch]")
-    device = key_cache.device
-    if not (value_cache.device == block_tables.device == token_offsets.device == key.device == value.device == device):
-        raise ValueError("batch KV tensors must share the cache device")
+    device = _device_of((key_cache, value_cache, block_tables, token_offsets, key, value), ValueError,
+                        "batch KV tensors must share the cache device")
     width = block_tables.shape[1]
     if validate and batch:
         if bool(((token_offsets < 0) | (token_offsets >= width * block_size)).any()):
@@ -168,7 +177,8 @@ def write_kv_cache_batch_int4(key_cache, value_cache, block_tables, token_offset
             key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), token_offsets.data_ptr(),
             key.data_ptr(), value.data_ptr(), batch, width, num_blocks, block_size, kv_heads, key.shape[2], key_stride,
             value_stride, _lib.DTYPE_CODES[key.dtype], _lib.stream_of(device))
-    _lib.check(status, "write_kv_cache_batch_int4")
+    if status:
+        _lib.check(status, "write_kv_cache_batch_int4")
 
 
 def read_kv_cache_slots_int4(key_cache, value_cache, slot_mapping, block_size, head_dim, *, dtype=torch.float32,
@@ -180,13 +190,13 @@ def read_kv_cache_slots_int4(key_cache, value_cache, slot_mapping, block_size, h
     """
     _backend(backend)
     num_blocks, kv_heads = _check_pools(key_cache, value_cache, block_size, head_dim)
-    if dtype not in _lib.DTYPE_CODES:
+    code = _lib.DTYPE_CODES.get(dtype)
+    if code is None:
         raise ValueError("packed KV requires FP32/FP16/BF16")
-    if slot_mapping.ndim != 1 or slot_mapping.dtype != torch.int64 or not slot_mapping.is_contiguous():
+    if slot_mapping.ndim != 1 or slot_mapping.dtype is not torch.int64 or not slot_mapping.is_contiguous():
         raise ValueError("slot_mapping must be contiguous int64 [tokens]")
-    device = key_cache.device
-    if value_cache.device != device or slot_mapping.device != device:
-        raise ValueError("packed KV tensors and slots must share the cache device")
+    device = _device_of((key_cache, value_cache, slot_mapping), ValueError,
+                        "packed KV tensors and slots must share the cache device")
     if validate and slot_mapping.numel():
         if bool(((slot_mapping < 0) | (slot_mapping >= num_blocks * block_size)).any()):
             raise ValueError("KV slot is outside cache capacity")
@@ -201,40 +211,49 @@ def read_kv_cache_slots_int4(key_cache, value_cache, slot_mapping, block_size, h
     with _lib.on_device(device):
         status = lib.minikv_kv_gather_slots_int4(
             key_cache.data_ptr(), value_cache.data_ptr(), slot_mapping.data_ptr(), key.data_ptr(), value.data_ptr(),
-            tokens, num_blocks, block_size, kv_heads, head_dim, _lib.DTYPE_CODES[dtype], _lib.stream_of(device))
-    _lib.check(status, "read_kv_cache_slots_int4")
+            tokens, num_blocks, block_size, kv_heads, head_dim, code, _lib.stream_of(device))
+    if status:
+        _lib.check(status, "read_kv_cache_slots_int4")
     return key, value
 
 
 # ------------------------------------------------------------------ decode
 
-_WS_BYTES: dict = {}
-_TICKETS: dict = {}
-_OLD_TICKETS: list = []
+_NEEDS: dict = {}
+_SCRATCH: dict = {}
+_OLD_SCRATCH: list = []
 
 
-def _tickets(device, stream, count):
-    """Zero counters of a page decode.  Every launch leaves them zero, so calls on one stream share them.
+def _scratch(device, stream, tickets, need):
+    """(ticket counters, workspace) of a page decode.
 
-    A captured graph may run beside other work of its stream, so it gets counters
-    of its own, zeroed inside the graph.
+    Every launch leaves the counters zero, whatever its shape, and the workspace
+    may hold anything, so the eager calls on one stream, which follow one another,
+    share them.  A captured graph may run beside other work of its stream: it gets
+    its own, from the graph's memory, zeroed inside the graph.
     """
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(count, dtype=torch.int32, device=device)
+        return (torch.zeros(tickets, dtype=torch.int32, device=device),
+                torch.empty(need, dtype=torch.uint8, device=device))
     key = (device.index, stream)
-    held = _TICKETS.get(key)
-    if held is None or held.numel() < count:
+    held = _SCRATCH.get(key)
+    if held is None or held[0].numel() < tickets or held[1].numel() < need:
         if held is not None:
-            _OLD_TICKETS.append(held)  # a launch in flight may still use it
-        held = _TICKETS[key] = torch.zeros(max(count, 4096), dtype=torch.int32, device=device)
+            _OLD_SCRATCH.append(held)  # a launch in flight may still use it
+            tickets, need = max(tickets, 2 * held[0].numel()), max(need, 2 * held[1].numel())
+        held = _SCRATCH[key] = (torch.zeros(max(tickets, 4096), dtype=torch.int32, device=device),
+                                torch.empty(need, dtype=torch.uint8, device=device))
     return held
 
 
 def _check_selected(selected, block_tables, context_lens, kv_heads, block_size, validate):
-    _require(selected.dtype == torch.int64 and selected.is_contiguous(), "selected must be contiguous int64")
-    _require(selected.device == block_tables.device, "all inputs must be on the same CUDA device")
-    _require(selected.dim() == 3 and selected.shape[:2] == (block_tables.shape[0], kv_heads) and selected.shape[2] > 0,
-             "selected must be [batch, kv_heads, blocks]")
+    if selected.dtype is not torch.int64 or not selected.is_contiguous():
+        raise RuntimeError("selected must be contiguous int64")
+    if selected.get_device() != block_tables.get_device():
+        raise RuntimeError("all inputs must be on the same CUDA device")
+    shape = selected.shape
+    if len(shape) != 3 or shape[0] != block_tables.shape[0] or shape[1] != kv_heads or shape[2] <= 0:
+        raise RuntimeError("selected must be [batch, kv_heads, blocks]")
     if validate:
         blocks = ((context_lens + block_size - 1) // block_size)[:, None, None]
         _require(not bool(((selected < -1) | (selected >= blocks)).any()), "selected block out of range")
@@ -247,20 +266,26 @@ def _check_selected(selected, block_tables, context_lens, kv_heads, block_size, 
 def _decode_pages(entry, sizer, query, key_cache, value_cache, block_tables, context_lens, selected, block_size,
                   num_blocks, kv_heads, validate):
     """Metadata checks and launch shared by the decodes over page lists."""
-    device = query.device
-    _require(query.is_contiguous() and key_cache.is_contiguous() and value_cache.is_contiguous()
-             and block_tables.is_contiguous() and context_lens.is_contiguous(), "inputs must be contiguous")
-    _require(key_cache.device == value_cache.device == block_tables.device == context_lens.device == device,
-             "all inputs must be on the same CUDA device")
-    _require(block_tables.dtype == torch.int64 and context_lens.dtype == torch.int64, "metadata must be int64")
+    if not (query.is_contiguous() and key_cache.is_contiguous() and value_cache.is_contiguous()
+            and block_tables.is_contiguous() and context_lens.is_contiguous()):
+        raise RuntimeError("inputs must be contiguous")
+    device = _device_of((query, key_cache, value_cache, block_tables, context_lens), RuntimeError,
+                        "all inputs must be on the same CUDA device")
+    if block_tables.dtype is not torch.int64 or context_lens.dtype is not torch.int64:
+        raise RuntimeError("metadata must be int64")
     batch, heads, dim = query.shape
-    _require(batch > 0 and heads > 0, "empty batch/heads/cache")
-    _require(heads % kv_heads == 0, "head dimension or GQA mismatch")
-    _require(block_tables.dim() == 2 and block_tables.shape[0] == batch and block_tables.shape[1] > 0,
-             "invalid block table")
-    _require(context_lens.dim() == 1 and context_lens.shape[0] == batch, "invalid context lengths")
-    width = block_tables.shape[1]
-    _require(width * block_size <= 1048576, "maximum table capacity is 1M tokens")
+    if batch <= 0 or heads <= 0:
+        raise RuntimeError("empty batch/heads/cache")
+    if heads % kv_heads:
+        raise RuntimeError("head dimension or GQA mismatch")
+    table = block_tables.shape
+    if len(table) != 2 or table[0] != batch or table[1] <= 0:
+        raise RuntimeError("invalid block table")
+    if context_lens.shape != (batch,):
+        raise RuntimeError("invalid context lengths")
+    width = table[1]
+    if width * block_size > 1048576:
+        raise RuntimeError("maximum table capacity is 1M tokens")
     if validate:
         _require(not bool(((context_lens <= 0) | (context_lens > width * block_size)).any()),
                  "invalid context length")
@@ -268,30 +293,29 @@ def _decode_pages(entry, sizer, query, key_cache, value_cache, block_tables, con
         active = positions.unsqueeze(0) < context_lens.unsqueeze(1)
         _require(not bool((((block_tables < 0) | (block_tables >= num_blocks)) & active).any()),
                  "physical block id out of range")
-    take = 0
+    take, listed = 0, None
     if selected is not None:
         _check_selected(selected, block_tables, context_lens, kv_heads, block_size, validate)
-        take = selected.shape[2]
+        take, listed = selected.shape[2], selected.data_ptr()
     lib = _lib.load()
     code = _lib.DTYPE_CODES[query.dtype]
     with _lib.on_device(device):
         key = (sizer, device.index, batch, heads, kv_heads, dim, code)
-        need = _WS_BYTES.get(key)
+        need = _NEEDS.get(key)
         if need is None:
             need = getattr(lib, sizer)(batch, heads, kv_heads, dim, num_blocks, block_size, width, code)
             if need < 0:
                 _lib.check(_lib.EINVAL, entry)
-            _WS_BYTES[key] = need
+            _NEEDS[key] = need
         stream = _lib.stream_of(device)
-        tickets = _tickets(device, stream, batch * kv_heads * ((heads // kv_heads + 7) // 8))
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        tickets, workspace = _scratch(device, stream, batch * kv_heads * ((heads // kv_heads + 7) // 8), need)
         out = torch.empty_like(query)
         status = getattr(lib, entry)(
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
-            context_lens.data_ptr(), None if selected is None else selected.data_ptr(), out.data_ptr(),
-            tickets.data_ptr(), workspace.data_ptr(), need, batch, heads, kv_heads, dim, num_blocks, block_size, width,
-            take, code, stream)
-    _lib.check(status, entry)
+            context_lens.data_ptr(), listed, out.data_ptr(), tickets.data_ptr(), workspace.data_ptr(), need, batch,
+            heads, kv_heads, dim, num_blocks, block_size, width, take, code, stream)
+    if status:
+        _lib.check(status, entry)
     return out
 
 
@@ -308,9 +332,12 @@ def paged_attention_int4(query, key_cache, value_cache, block_tables, context_le
     fits its range.  Returns ``[B, Hq, D]`` in the query dtype.
     """
     check_backend(backend)
-    _require(query.is_cuda, "query must be CUDA")
-    _require(query.dim() == 3, "invalid query/cache shapes")
-    _require(query.dtype in _QUERY_DTYPES, "a 4-bit KV pool needs an FP16/BF16 query")
+    if not query.is_cuda:
+        raise RuntimeError("query must be CUDA")
+    if query.dim() != 3:
+        raise RuntimeError("invalid query/cache shapes")
+    if query.dtype not in _QUERY_DTYPES:
+        raise RuntimeError("a 4-bit KV pool needs an FP16/BF16 query")
     num_blocks, kv_heads = _check_pools(key_cache, value_cache, block_size, query.shape[2], RuntimeError)
     return _decode_pages("minikv_paged_decode_int4", "minikv_paged_decode_int4_workspace_bytes", query, key_cache,
                          value_cache, block_tables, context_lens, selected, block_size, num_blocks, kv_heads, validate)
@@ -371,5 +398,6 @@ def paged_prefill_attention_int4(q, key_cache, value_cache, cu_seqlens_q, query_
             query_starts.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), output.data_ptr(), tokens,
             requests, q.shape[1], kv_heads, q.shape[2], num_blocks, block_size, width, bound,
             _lib.DTYPE_CODES[q.dtype], _lib.stream_of(q.device))
-    _lib.check(status, "paged_prefill_attention_int4")
+    if status:
+        _lib.check(status, "paged_prefill_attention_int4")
     return output

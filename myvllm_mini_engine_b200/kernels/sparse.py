@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .int4 import INT4_HEAD_DIMS, _decode_pages, int4_page_bytes
+from .int4 import _QUERY_DTYPES, INT4_HEAD_DIMS, _decode_pages, _device_of, int4_page_bytes
 from .paged import _require, check_backend
 
 _INT4 = 3  # MINIKV_INT4
@@ -38,12 +38,13 @@ def block_bounds_bytes(head_dim):
 
 def _check_bounds(bounds):
     """``(num_blocks, kv_heads, head_dim)`` of a bounds tensor."""
-    _require(bounds.dim() == 3 and bounds.dtype == torch.uint8 and bounds.is_contiguous() and bounds.numel() > 0,
-             "block bounds must be contiguous uint8 [pages, kv_heads, 2 * head_dim + 16]")
-    dim = (bounds.shape[2] - 16) // 2
-    _require(dim in INT4_HEAD_DIMS and bounds.shape[2] == 2 * dim + 16,
-             "block bounds need head_dim 32, 64, 96, 128, 192 or 256")
-    return bounds.shape[0], bounds.shape[1], dim
+    shape = bounds.shape
+    if len(shape) != 3 or bounds.dtype is not torch.uint8 or not bounds.is_contiguous() or 0 in shape:
+        raise RuntimeError("block bounds must be contiguous uint8 [pages, kv_heads, 2 * head_dim + 16]")
+    dim = (shape[2] - 16) // 2
+    if dim not in INT4_HEAD_DIMS or shape[2] != 2 * dim + 16:
+        raise RuntimeError("block bounds need head_dim 32, 64, 96, 128, 192 or 256")
+    return shape[0], shape[1], dim
 
 
 def update_block_bounds(bounds, key_cache, block_tables, query_starts, context_lens, block_size, *, backend="cuda",
@@ -60,27 +61,32 @@ def update_block_bounds(bounds, key_cache, block_tables, query_starts, context_l
     """
     check_backend(backend)
     num_blocks, kv_heads, dim = _check_bounds(bounds)
-    if key_cache.dtype == torch.uint8:
+    if type(block_size) is not int or block_size <= 0:
+        raise RuntimeError("block size mismatch")
+    if key_cache.dtype is torch.uint8:
         pool = _INT4
-        _require(key_cache.dim() == 3 and type(block_size) is int and block_size > 0
-                 and key_cache.shape == (num_blocks, kv_heads, int4_page_bytes(block_size, dim)),
-                 "4-bit key cache must be [pages, kv_heads, page_bytes] matching the bounds")
+        if key_cache.shape != (num_blocks, kv_heads, int4_page_bytes(block_size, dim)):
+            raise RuntimeError("4-bit key cache must be [pages, kv_heads, page_bytes] matching the bounds")
     else:
         pool = _lib.dtype_code(key_cache.dtype)
-        _require(key_cache.dim() == 4 and type(block_size) is int
-                 and key_cache.shape == (num_blocks, block_size, kv_heads, dim),
-                 "key cache must be [pages, block_size, kv_heads, head_dim] matching the bounds")
-    _require(bounds.is_cuda, "bounds must be CUDA")
-    tensors = (key_cache, block_tables, query_starts, context_lens)
-    _require(all(t.device == bounds.device for t in tensors), "all inputs must be on the same CUDA device")
-    _require(all(t.is_contiguous() for t in tensors), "inputs must be contiguous")
-    _require(all(t.dtype == torch.int64 for t in tensors[1:]), "metadata must be int64")
-    requests = query_starts.shape[0] if query_starts.dim() == 1 else -1
-    _require(requests >= 0 and context_lens.dim() == 1 and context_lens.shape[0] == requests
-             and block_tables.dim() == 2 and block_tables.shape[0] == requests and block_tables.shape[1] > 0,
-             "block bounds metadata shapes do not match request count")
-    width = block_tables.shape[1]
-    _require(width * block_size <= 1048576, "maximum table capacity is 1M tokens")
+        if key_cache.shape != (num_blocks, block_size, kv_heads, dim):
+            raise RuntimeError("key cache must be [pages, block_size, kv_heads, head_dim] matching the bounds")
+    if not bounds.is_cuda:
+        raise RuntimeError("bounds must be CUDA")
+    device = _device_of((bounds, key_cache, block_tables, query_starts, context_lens), RuntimeError,
+                        "all inputs must be on the same CUDA device")
+    if not (key_cache.is_contiguous() and block_tables.is_contiguous() and query_starts.is_contiguous()
+            and context_lens.is_contiguous()):
+        raise RuntimeError("inputs must be contiguous")
+    if (block_tables.dtype is not torch.int64 or query_starts.dtype is not torch.int64
+            or context_lens.dtype is not torch.int64):
+        raise RuntimeError("metadata must be int64")
+    if (query_starts.dim() != 1 or context_lens.shape != query_starts.shape or block_tables.dim() != 2
+            or block_tables.shape[0] != query_starts.shape[0] or block_tables.shape[1] <= 0):
+        raise RuntimeError("block bounds metadata shapes do not match request count")
+    requests, width = block_tables.shape
+    if width * block_size > 1048576:
+        raise RuntimeError("maximum table capacity is 1M tokens")
     if validate and requests:
         _require(not bool(((query_starts < 0) | (query_starts > context_lens)
                            | (context_lens > width * block_size)).any()), "invalid context length")
@@ -93,12 +99,13 @@ def update_block_bounds(bounds, key_cache, block_tables, query_starts, context_l
         return
     longest = width * block_size if max_query_len is None else int(max_query_len)
     lib = _lib.load()
-    with _lib.on_device(bounds.device):
+    with _lib.on_device(device):
         status = lib.minikv_block_bounds_update(
             bounds.data_ptr(), key_cache.data_ptr(), block_tables.data_ptr(), query_starts.data_ptr(),
             context_lens.data_ptr(), requests, width, num_blocks, block_size, kv_heads, dim, longest, pool,
-            _lib.stream_of(bounds.device))
-    _lib.check(status, "update_block_bounds")
+            _lib.stream_of(device))
+    if status:
+        _lib.check(status, "update_block_bounds")
 
 
 def read_block_bounds(bounds, block_ids, *, validate=True):
@@ -107,22 +114,24 @@ def read_block_bounds(bounds, block_ids, *, validate=True):
     A block outside the pool gives zeros (refused with ``validate``).
     """
     num_blocks, kv_heads, dim = _check_bounds(bounds)
-    _require(bounds.is_cuda and block_ids.device == bounds.device, "all inputs must be on the same CUDA device")
-    _require(block_ids.dim() == 1 and block_ids.dtype == torch.int64 and block_ids.is_contiguous(),
-             "block ids must be contiguous int64 [n]")
+    if not bounds.is_cuda or block_ids.get_device() != bounds.get_device():
+        raise RuntimeError("all inputs must be on the same CUDA device")
+    if block_ids.dim() != 1 or block_ids.dtype is not torch.int64 or not block_ids.is_contiguous():
+        raise RuntimeError("block ids must be contiguous int64 [n]")
     count = block_ids.shape[0]
     if validate and count:
         _require(not bool(((block_ids < 0) | (block_ids >= num_blocks)).any()), "physical block id out of range")
-    lower = torch.empty((count, kv_heads, dim), dtype=torch.float32, device=bounds.device)
+    device = bounds.device
+    lower = torch.empty((count, kv_heads, dim), dtype=torch.float32, device=device)
     upper = torch.empty_like(lower)
     if count == 0:
         return lower, upper
     lib = _lib.load()
-    with _lib.on_device(bounds.device):
+    with _lib.on_device(device):
         status = lib.minikv_block_bounds_read(bounds.data_ptr(), block_ids.data_ptr(), count, lower.data_ptr(),
-                                              upper.data_ptr(), num_blocks, kv_heads, dim,
-                                              _lib.stream_of(bounds.device))
-    _lib.check(status, "read_block_bounds")
+                                              upper.data_ptr(), num_blocks, kv_heads, dim, _lib.stream_of(device))
+    if status:
+        _lib.check(status, "read_block_bounds")
     return lower, upper
 
 
@@ -137,26 +146,31 @@ def select_blocks(query, bounds, block_tables, context_lens, block_size, max_blo
     of them.  The bounds of every block below ``context_lens`` must be up to date.
     """
     check_backend(backend)
-    _require(query.is_cuda, "query must be CUDA")
+    if not query.is_cuda:
+        raise RuntimeError("query must be CUDA")
     num_blocks, kv_heads, dim = _check_bounds(bounds)
-    _require(query.dim() == 3 and query.shape[2] == dim and query.shape[1] % kv_heads == 0 and query.numel() > 0,
-             "head dimension or GQA mismatch")
+    shape = query.shape
+    if len(shape) != 3 or shape[2] != dim or shape[1] % kv_heads or 0 in shape:
+        raise RuntimeError("head dimension or GQA mismatch")
+    batch, heads, _ = shape
     code = _lib.dtype_code(query.dtype)
-    device = query.device
-    _require(bounds.device == block_tables.device == context_lens.device == device,
-             "all inputs must be on the same CUDA device")
-    _require(query.is_contiguous() and block_tables.is_contiguous() and context_lens.is_contiguous(),
-             "inputs must be contiguous")
-    _require(block_tables.dtype == torch.int64 and context_lens.dtype == torch.int64, "metadata must be int64")
-    batch = query.shape[0]
-    _require(block_tables.dim() == 2 and block_tables.shape[0] == batch and block_tables.shape[1] > 0,
-             "invalid block table")
-    _require(context_lens.dim() == 1 and context_lens.shape[0] == batch, "invalid context lengths")
-    _require(type(block_size) is int and block_size > 0, "block size mismatch")
+    device = _device_of((query, bounds, block_tables, context_lens), RuntimeError,
+                        "all inputs must be on the same CUDA device")
+    if not (query.is_contiguous() and block_tables.is_contiguous() and context_lens.is_contiguous()):
+        raise RuntimeError("inputs must be contiguous")
+    if block_tables.dtype is not torch.int64 or context_lens.dtype is not torch.int64:
+        raise RuntimeError("metadata must be int64")
+    if block_tables.dim() != 2 or block_tables.shape[0] != batch or block_tables.shape[1] <= 0:
+        raise RuntimeError("invalid block table")
+    if context_lens.shape != (batch,):
+        raise RuntimeError("invalid context lengths")
+    if type(block_size) is not int or block_size <= 0:
+        raise RuntimeError("block size mismatch")
     width = block_tables.shape[1]
-    _require(width * block_size <= 1048576, "maximum table capacity is 1M tokens")
-    _require(max_blocks > 0 and sink_blocks >= 0 and recent_blocks >= 0 and sink_blocks + recent_blocks <= max_blocks,
-             "max_blocks must be positive and hold the sink and recent blocks")
+    if width * block_size > 1048576:
+        raise RuntimeError("maximum table capacity is 1M tokens")
+    if max_blocks <= 0 or sink_blocks < 0 or recent_blocks < 0 or sink_blocks + recent_blocks > max_blocks:
+        raise RuntimeError("max_blocks must be positive and hold the sink and recent blocks")
     if validate:
         _require(not bool(((context_lens <= 0) | (context_lens > width * block_size)).any()),
                  "invalid context length")
@@ -170,9 +184,10 @@ def select_blocks(query, bounds, block_tables, context_lens, block_size, max_blo
         selected = torch.empty((batch, kv_heads, max_blocks), dtype=torch.int64, device=device)
         status = lib.minikv_select_blocks(
             query.data_ptr(), bounds.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), selected.data_ptr(),
-            workspace.data_ptr(), workspace.numel() * 4, batch, query.shape[1], kv_heads, dim, num_blocks, block_size,
+            workspace.data_ptr(), workspace.numel() * 4, batch, heads, kv_heads, dim, num_blocks, block_size,
             width, max_blocks, sink_blocks, recent_blocks, code, _lib.stream_of(device))
-    _lib.check(status, "select_blocks")
+    if status:
+        _lib.check(status, "select_blocks")
     return selected
 
 
@@ -187,15 +202,22 @@ def paged_attention_selected(query, key_cache, value_cache, block_tables, contex
     is masked gives zeros.  Returns ``[B, Hq, D]``.
     """
     check_backend(backend)
-    _require(query.is_cuda, "query must be CUDA")
-    _require(query.dim() == 3 and key_cache.dim() == 4 and value_cache.shape == key_cache.shape
-             and key_cache.numel() > 0, "invalid query/cache shapes")
-    _require(query.dtype in (torch.float16, torch.bfloat16), "FP16/BF16 required")
-    _require(key_cache.dtype == query.dtype and value_cache.dtype == query.dtype, "cache dtype mismatch")
-    num_blocks, bs, kv_heads, dim = key_cache.shape
-    _require(type(block_size) is int and bs == block_size, "block size mismatch")
-    _require(query.shape[2] == dim, "head dimension or GQA mismatch")
-    _require(dim in INT4_HEAD_DIMS, "selected blocks: supported head_dim: 32,64,96,128,192,256")
+    if not query.is_cuda:
+        raise RuntimeError("query must be CUDA")
+    shape = key_cache.shape
+    if query.dim() != 3 or len(shape) != 4 or value_cache.shape != shape or 0 in shape:
+        raise RuntimeError("invalid query/cache shapes")
+    if query.dtype not in _QUERY_DTYPES:
+        raise RuntimeError("FP16/BF16 required")
+    if key_cache.dtype is not query.dtype or value_cache.dtype is not query.dtype:
+        raise RuntimeError("cache dtype mismatch")
+    num_blocks, bs, kv_heads, dim = shape
+    if type(block_size) is not int or bs != block_size:
+        raise RuntimeError("block size mismatch")
+    if query.shape[2] != dim:
+        raise RuntimeError("head dimension or GQA mismatch")
+    if dim not in INT4_HEAD_DIMS:
+        raise RuntimeError("selected blocks: supported head_dim: 32,64,96,128,192,256")
     return _decode_pages("minikv_paged_decode_selected", "minikv_paged_decode_selected_workspace_bytes", query,
                          key_cache, value_cache, block_tables, context_lens, selected, block_size, num_blocks,
                          kv_heads, validate)
