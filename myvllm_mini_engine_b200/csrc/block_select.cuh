@@ -364,6 +364,55 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) score_blocks_kernel(con
     const int first = (int)(blockIdx.x - b * chunks) * p.span;
     if (first >= n || n <= p.take) return;  // a request with no more blocks than are taken needs no scores
     const int h0 = blockIdx.y * kScoreHeads, nh = min(kScoreHeads, p.kv_heads - h0);
+    // ---- blocks: warp w takes blocks w, w + 8, ... of the span, AHEAD at a time, the next ones loaded
+    // while these are scored (the first while the query's codes are made); lane x looks up the page of
+    // the warp's next x-th block for 32 of them at once
+    constexpr int AHEAD = 2;
+    const int sub = lane % LPH, part = lane / LPH;
+    const bool active = sub * 16 < 2 * D;
+    const int last = min(n, first + p.span), mine = (last - first - warp + 7) / 8;
+    const int64_t* table = p.tables + b * p.width + first + warp;
+    const int recent_from = n - p.recent;
+    const int64_t stride = p.kv_heads * (int64_t)REC;
+    const unsigned char* lane_at = p.bounds + (int64_t)(h0 + part) * REC + (active ? sub * 16 : 0);
+    // The sums of the passes are halved across the lanes of a head as they are added up, so that a lane
+    // ends with the sum of one pass: head my_head, complete in the lanes that are `out`.
+    int my_pass = 0;
+#pragma unroll
+    for (int half = PASSES / 2, m = LPH / 2; half > 0; half /= 2, m /= 2) my_pass += (lane & m) ? half : 0;
+    const int my_head = my_pass * HPW + part;
+    const bool out = sub % (LPH / PASSES) == 0 && my_head < nh;
+    const unsigned char* scale_at = p.bounds + (int64_t)(h0 + min(my_head, nh - 1)) * REC + 2 * D;
+    struct Records {
+        int4 v[AHEAD][PASSES];
+        float scale[AHEAD];
+        bool ok[AHEAD];
+    };
+    int64_t page = 0;
+    auto load = [&](Records& r, int k0) {
+        if (k0 % 32 == 0) {
+            const int k = k0 + lane;
+            page = k < mine ? table[8 * k] : -1;
+            if (page >= p.num_blocks) page = -1;
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            const int64_t id = __shfl_sync(0xffffffffu, page, (k0 + a) % 32);
+            r.ok[a] = id >= 0;
+            const int64_t off = (r.ok[a] ? id : 0) * stride;
+            const unsigned char* rec = lane_at + off;
+            r.scale[a] = __ldg(reinterpret_cast<const float*>(scale_at + off));
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                // a group of fewer heads reads its first again
+                const unsigned char* at = rec + (FULL || i * HPW + part < nh ? i * HPW * REC : -part * REC);
+                const uint4 w = ld_global_nc(at);
+                r.v[a][i] = make_int4((int)w.x, (int)w.y, (int)w.z, (int)w.w);
+            }
+        }
+    };
+    Records even, odd;
+    load(even, 0);
     // ---- the query's codes
     if (tid < kScoreHeads) tops[tid] = 0;
     __syncthreads();
@@ -396,64 +445,46 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) score_blocks_kernel(con
         codes[h][d] = (signed char)min(127, max(-127, (int)c));
     }
     __syncthreads();
-    const int sub = lane % LPH, part = lane / LPH;
-    const bool active = sub * 16 < 2 * D;
     int4 qc[PASSES];
 #pragma unroll
     for (int i = 0; i < PASSES; ++i)
         qc[i] = active ? *reinterpret_cast<const int4*>(&codes[i * HPW + part][sub * 16]) : make_int4(0, 0, 0, 0);
-    // ---- blocks: warp w takes blocks w, w + 8, ... of the span, AHEAD of them in flight; lane x looks
-    // up the page of the warp's next x-th block for 32 of them at once
-    constexpr int AHEAD = D <= 128 ? 4 : 2;
-    const int last = min(n, first + p.span), mine = (last - first - warp + 7) / 8;
-    const int64_t* table = p.tables + b * p.width + first + warp;
-    const int recent_from = n - p.recent;
-    const int64_t stride = p.kv_heads * (int64_t)REC;
-    const unsigned char* lane_at = p.bounds + (int64_t)(h0 + part) * REC + (active ? sub * 16 : 0);
-    const int to_scale = 2 * D - (active ? sub * 16 : 0);
-    int64_t page = 0;
-    for (int k0 = 0; k0 < mine; k0 += AHEAD) {
-        if (k0 % 32 == 0) {
-            const int k = k0 + lane;
-            page = k < mine ? table[8 * k] : -1;
-            if (page >= p.num_blocks) page = -1;
-        }
-        int4 v[AHEAD][PASSES];
-        float scale[AHEAD][PASSES];
-        bool ok[AHEAD];
+    auto score = [&](const Records& r, int k0) {
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
-            const int64_t id = __shfl_sync(0xffffffffu, page, (k0 + a) % 32);
-            ok[a] = id >= 0;
-            const unsigned char* rec = lane_at + (ok[a] ? id : 0) * stride;
+            int dot[PASSES];
 #pragma unroll
             for (int i = 0; i < PASSES; ++i) {
-                // a group of fewer heads reads its first again
-                const unsigned char* at = rec + (FULL || i * HPW + part < nh ? i * HPW * REC : -part * REC);
-                const uint4 w = ld_global_nc(at);
-                v[a][i] = make_int4((int)w.x, (int)w.y, (int)w.z, (int)w.w);
-                scale[a][i] = __ldg(reinterpret_cast<const float*>(at + to_scale));
+                dot[i] = __dp4a(r.v[a][i].x, qc[i].x, 0);
+                dot[i] = __dp4a(r.v[a][i].y, qc[i].y, dot[i]);
+                dot[i] = __dp4a(r.v[a][i].z, qc[i].z, dot[i]);
+                dot[i] = __dp4a(r.v[a][i].w, qc[i].w, dot[i]);
             }
-        }
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            const int j = first + warp + 8 * (k0 + a);
-            const bool forced = j < p.sink || j >= recent_from;
+            for (int half = PASSES / 2, m = LPH / 2; m > 0; half /= 2, m /= 2) {
+                const bool upper = lane & m;
 #pragma unroll
-            for (int i = 0; i < PASSES; ++i) {
-                int dot = __dp4a(v[a][i].x, qc[i].x, 0);
-                dot = __dp4a(v[a][i].y, qc[i].y, dot);
-                dot = __dp4a(v[a][i].z, qc[i].z, dot);
-                dot = __dp4a(v[a][i].w, qc[i].w, dot);
-#pragma unroll
-                for (int m = LPH / 2; m > 0; m >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, m);
-                if (sub == 0 && k0 + a < mine) {
-                    const float s = __fmul_rn((float)dot, scale[a][i]);
-                    const uint32_t key = forced ? 0xffffffffu : isnan(s) ? 1u : score_key(s);
-                    found[i * HPW + part][j - first] = ok[a] ? key : 0u;
+                for (int i = 0; i < (half > 0 ? half : 1); ++i) {
+                    const int keep = half > 0 && upper ? dot[i + half] : dot[i];
+                    const int give = half > 0 && !upper ? dot[i + half] : dot[i];
+                    dot[i] = keep + __shfl_xor_sync(0xffffffffu, give, m);
                 }
             }
+            if (out && k0 + a < mine) {
+                const int j = first + warp + 8 * (k0 + a);
+                const float s = __fmul_rn((float)dot[0], r.scale[a]);
+                uint32_t key = isnan(s) ? 1u : score_key(s);
+                if (j < p.sink || j >= recent_from) key = 0xffffffffu;
+                found[my_head][j - first] = r.ok[a] ? key : 0u;
+            }
         }
+    };
+#pragma unroll 1
+    for (int k0 = 0; k0 < mine; k0 += 2 * AHEAD) {
+        if (k0 + AHEAD < mine) load(odd, k0 + AHEAD);
+        score(even, k0);
+        if (k0 + 2 * AHEAD < mine) load(even, k0 + 2 * AHEAD);
+        if (k0 + AHEAD < mine) score(odd, k0 + AHEAD);
     }
     __syncthreads();
     for (int h = 0; h < nh; ++h)
@@ -469,21 +500,24 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) score_blocks_kernel(con
 constexpr int kSelectThreads = 512;
 constexpr int kSelectHeld = 24576;  // keys in shared memory (96 KB)
 
-// Sum over the CTA, in one barrier: `turn` alternates between two sets of warp sums.
-__device__ __forceinline__ int block_sum(int x, int (*sums)[32], int turn) {
+// Sums of x and y over the CTA, in one barrier: `turn` alternates between two sets of warp sums.
+__device__ __forceinline__ uint2 block_sum2(uint32_t x, uint32_t y, uint2 (*sums)[32], int turn) {
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     x = __reduce_add_sync(0xffffffffu, x);
-    if (lane == 0) sums[turn & 1][threadIdx.x >> 5] = x;
+    y = __reduce_add_sync(0xffffffffu, y);
+    if (lane == 0) sums[turn & 1][threadIdx.x >> 5] = make_uint2(x, y);
     __syncthreads();
-    return __reduce_add_sync(0xffffffffu, lane < warps ? sums[turn & 1][lane] : 0);
+    const uint2 s = lane < warps ? sums[turn & 1][lane] : make_uint2(0u, 0u);
+    return make_uint2(__reduce_add_sync(0xffffffffu, s.x), __reduce_add_sync(0xffffffffu, s.y));
 }
 
 // Requests of up to 4096 blocks: a thread holds KEYS consecutive keys in registers, and the
-// take-th largest is found bit by bit, a count and a barrier each, until a value is met that exactly
-// `take` keys reach (a score's 32 bits rarely tie).
+// take-th largest is found two bits at a time, three counts and a barrier each, until a value is met
+// that exactly `take` keys reach (a score's 32 bits rarely tie).
 template <int KEYS>
 __global__ void __launch_bounds__(512) select_few_kernel(const SelectParams p) {
     __shared__ int counts[2][32];
+    __shared__ uint2 sums[2][32];
     griddep_wait();
     griddep_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
@@ -510,23 +544,25 @@ __global__ void __launch_bounds__(512) select_few_kernel(const SelectParams p) {
     int above = 0;  // keys over it
     int turn = 0;
     if (!all) {
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t probe = threshold | (1u << bit);
-            int count = 0;
-            if constexpr (KEYS == 1) {
-                count = __syncthreads_count(key[0] >= probe);
-            } else {
+        const uint32_t take = (uint32_t)p.take;
+        for (int shift = 30; shift >= 0; shift -= 2) {
+            const uint32_t one = threshold | (1u << shift), two = threshold | (2u << shift), three = threshold | (3u << shift);
+            uint32_t c12 = 0, c3 = 0;  // counts of two probes share a word: a CTA has 4096 keys at most
 #pragma unroll
-                for (int i = 0; i < KEYS; ++i) count += key[i] >= probe;
-                count = block_sum(count, counts, turn++);
+            for (int i = 0; i < KEYS; ++i) {
+                c12 += (key[i] >= one ? 1u : 0u) + (key[i] >= two ? 65536u : 0u);
+                c3 += key[i] >= three;
             }
-            if (count >= p.take) threshold = probe;
-            if (count == p.take) break;  // exactly the keys from here on
+            const uint2 s = block_sum2(c12, c3, sums, turn++);
+            const uint32_t n1 = s.x & 0xffffu, n2 = s.x >> 16, n3 = s.y;
+            const uint32_t reached = n3 >= take ? n3 : n2 >= take ? n2 : n1;
+            threshold = n3 >= take ? three : n2 >= take ? two : n1 >= take ? one : threshold;
+            if (reached == take) break;  // exactly the keys from here on
         }
-        int count = 0;
+        uint32_t count = 0;
 #pragma unroll
         for (int i = 0; i < KEYS; ++i) count += key[i] > threshold;
-        above = block_sum(count, counts, turn++);
+        above = (int)block_sum2(count, 0u, sums, turn++).x;
     }
     __syncthreads();
     const int ties = all ? 0 : p.take - above;

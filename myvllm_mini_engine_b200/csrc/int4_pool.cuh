@@ -42,15 +42,19 @@ struct FastDiv {
 
 constexpr float kInt4StepMin = 1.f / 16777216.f;  // 2^-24, the smallest fp16
 
-// Lanes that share a row in the row kernels: 8 elements a lane, a power of two.
-constexpr int int4_row_lanes(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32; }
+// Blocks of 256 threads a SM in the row kernels: the grid fills the device once.
+constexpr int kInt4WriteBlocks = 4, kInt4ReadBlocks = 5;
 
-// 8 consecutive elements of a row, held as they came.  VEC: p is 16-byte aligned.
-template <typename T, bool VEC> struct Row8 {
-    uint4 v[8 / Elem<T>::kPerVec];
+// Lanes that share a row of D elements, E each: a power of two.
+constexpr int int4_row_lanes(int D, int E = 8) { return D / E <= 2 ? 2 : D / E <= 4 ? 4 : D / E <= 8 ? 8 : D / E <= 16 ? 16 : 32; }
+
+// 16 consecutive elements of a row, held as they came.  VEC: p is 16-byte aligned.
+template <typename T, bool VEC> struct RowPart {
+    static constexpr int VECS = 16 / Elem<T>::kPerVec;
+    uint4 v[VECS];
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-        for (int i = 0; i < 8 / Elem<T>::kPerVec; ++i) {
+        for (int i = 0; i < VECS; ++i) {
             if constexpr (VEC) {
                 v[i] = ld_global_nc(reinterpret_cast<const uint4*>(p) + i);
             } else {
@@ -61,17 +65,20 @@ template <typename T, bool VEC> struct Row8 {
             }
         }
     }
-    // Least and largest of the 8, and whether one is NaN, infinite or over 65504 in magnitude.
+    // Least and largest of the 16, and whether one is NaN, infinite or over 65504 in magnitude.
     __device__ __forceinline__ bool extremes(const float* f, float* lo, float* hi) const {
         bool odd;
         if constexpr (sizeof(T) == 2) {  // two elements an operation
             using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
             const Pair* x = reinterpret_cast<const Pair*>(v);
             const uint32_t zero = 0u;
-            Pair l = __hmin2(__hmin2(x[0], x[1]), __hmin2(x[2], x[3])), h = __hmax2(__hmax2(x[0], x[1]), __hmax2(x[2], x[3]));
-            Pair bad = *reinterpret_cast<const Pair*>(&zero);
+            Pair l = x[0], h = x[0], bad = __hmul2(x[0], *reinterpret_cast<const Pair*>(&zero));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) bad = __hfma2(x[i], *reinterpret_cast<const Pair*>(&zero), bad);
+            for (int i = 1; i < 8; ++i) {
+                l = __hmin2(l, x[i]);
+                h = __hmax2(h, x[i]);
+                bad = __hfma2(x[i], *reinterpret_cast<const Pair*>(&zero), bad);
+            }
             float a[2], b[2];
             Elem<T>::unpack(*reinterpret_cast<uint32_t*>(&l), a);
             Elem<T>::unpack(*reinterpret_cast<uint32_t*>(&h), b);
@@ -81,7 +88,7 @@ template <typename T, bool VEC> struct Row8 {
         } else {
             float bad = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 16; ++i) {
                 *lo = fminf(*lo, f[i]);
                 *hi = fmaxf(*hi, f[i]);
                 bad = fmaf(f[i], 0.f, bad);
@@ -92,7 +99,7 @@ template <typename T, bool VEC> struct Row8 {
     }
     __device__ __forceinline__ void values(float* f) const {
 #pragma unroll
-        for (int i = 0; i < 8 / Elem<T>::kPerVec; ++i) Elem<T>::load(v[i], f + i * Elem<T>::kPerVec);
+        for (int i = 0; i < VECS; ++i) Elem<T>::load(v[i], f + i * Elem<T>::kPerVec);
     }
 };
 
@@ -102,49 +109,66 @@ __device__ __forceinline__ uint32_t int4_code(float x, float base, float step) {
 }
 
 // Quantising write.  A unit is one row: (token, kv head, K or V); a group of
-// int4_row_lanes(D) lanes takes one, 8 elements a lane, so at D = 128 a warp
-// takes the K and the V row of a token's head.  The usual row costs an element
+// int4_row_lanes(D, 16) lanes takes one, 16 elements a lane, so at D = 128 a
+// warp takes the K and the V rows of two heads of a token (8 elements a lane,
+// twice the row's own work an element, took 46 us where this takes WRITE).  The usual row costs an element
 // a subtraction, two products with the rounded inverse of the step (a little
 // above and a little below it, each rounded to a whole number by an addition of
 // 1.5 2^23) and an addition into the word: where the two agree, so does the true
 // quotient.  Where they differ, and for rows with NaN, infinities, magnitudes
 // above 65504 or codes to clamp, the lane divides.
 template <typename T, int D, bool VEC, typename Rows>
-__global__ void __launch_bounds__(256) int4_write_kernel(
+__global__ void __launch_bounds__(256, kInt4WriteBlocks) int4_write_kernel(
     unsigned char* __restrict__ kc, unsigned char* __restrict__ vc, const T* __restrict__ k, const T* __restrict__ v,
     int64_t first_token, int64_t tokens, int kv_heads, FastDiv rows_of, FastDiv block_of, int64_t page_bytes,
     int64_t k_stride, int64_t v_stride, Rows map) {
     griddep_wait();
     griddep_launch_dependents();
-    constexpr int LPR = int4_row_lanes(D);
+    constexpr int LPR = int4_row_lanes(D, 16);
     constexpr float kRound = 12582912.f;  // 1.5 2^23
     const int sub = threadIdx.x % LPR;
-    const bool active = sub * 8 < D;
+    const bool active = sub * 16 < D;
     const uint32_t units = (uint32_t)(tokens * kv_heads * 2);
     const uint32_t groups = gridDim.x * (blockDim.x / LPR);
     // the loop's bound is the same for a whole warp: the shuffles need all lanes
     const uint32_t first = blockIdx.x * (blockDim.x / LPR) + threadIdx.x / LPR;
     const uint32_t warp_first = first - (threadIdx.x % 32) / LPR;
-    for (uint32_t off = 0; warp_first + off < units; off += groups) {
-        const uint32_t u = first + off;
+    struct Unit {
+        int64_t token;
+        uint32_t h;
+        bool in, which;
+    };
+    auto unit_at = [&](uint32_t u) {
         const bool in = u < units;
-        const uint32_t t = rows_of(in ? u : 0);
-        const uint32_t rest = in ? u - t * rows_of.d : 0, h = rest >> 1;
-        const bool which = rest & 1;
-        const int64_t token = first_token + t;
-        const int64_t row = in ? map(token) : -1;
-        Row8<T, VEC> raw;
-        float x[8];
+        const uint32_t t = rows_of(in ? u : 0), rest = in ? u - t * rows_of.d : 0;
+        return Unit{first_token + t, rest >> 1, in, (rest & 1) != 0};
+    };
+    auto source = [&](const Unit& n) {
+        return (n.which ? v + n.token * v_stride : k + n.token * k_stride) + (int64_t)n.h * D + sub * 16;
+    };
+    RowPart<T, VEC> ahead;  // the next row, loaded while this one is worked on
+    Unit next = unit_at(first);
+    if (active) ahead.load(source(next));
+    for (uint32_t off = 0; warp_first + off < units; off += groups) {
+        const Unit n = next;
+        const RowPart<T, VEC> raw = ahead;
+        const int64_t row = n.in ? map(n.token) : -1;
+        if (warp_first + off + groups < units) {
+            next = unit_at(first + off + groups);
+            if (active) ahead.load(source(next));
+        }
+        const uint32_t h = n.h;
+        const bool which = n.which;
+        float x[16];
         float lo = INFINITY, hi = -INFINITY;
         if (active) {
-            raw.load((which ? v + token * v_stride : k + token * k_stride) + (int64_t)h * D + sub * 8);
             raw.values(x);
             const bool odd = raw.extremes(x, &lo, &hi);
             if (odd) {
                 lo = INFINITY;
                 hi = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 16; ++i) {
                     x[i] = isnan(x[i]) ? 0.f : fminf(fmaxf(x[i], -65504.f), 65504.f);
                     lo = fminf(lo, x[i]);
                     hi = fmaxf(hi, x[i]);
@@ -166,22 +190,23 @@ __global__ void __launch_bounds__(256) int4_write_kernel(
         unsigned char* dst = (which ? vc : kc) + ((int64_t)page * kv_heads + h) * page_bytes;
         if (active) {
             const float over = inv * (1.f + 1.f / 1048576.f), under = inv * (1.f - 1.f / 1048576.f);
-            uint32_t word = 0, differ = 0;
+            uint32_t word[2] = {0u, 0u}, differ = 0;
             bool clamp = (lo - b) * inv < -0.49f || (hi - b) * inv > 15.49f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 16; ++i) {
                 const float d = x[i] - b;
                 const uint32_t up = __float_as_uint(fmaf(d, over, kRound)), down = __float_as_uint(fmaf(d, under, kRound));
                 differ |= up ^ down;
-                word += up << (4 * i);  // 0x4b400000 + code, the constants taken out below
+                word[i / 8] += up << (4 * (i % 8));  // 0x4b400000 + code, the constants taken out below
             }
-            word -= 0x3f400000u;  // 0x4b400000 (1 + 2^4 + 2^8 + ...) mod 2^32
+            word[0] -= 0x3f400000u;  // 0x4b400000 (1 + 2^4 + 2^8 + ...) mod 2^32
+            word[1] -= 0x3f400000u;
             if (differ != 0 || clamp) {
-                word = 0;
+                word[0] = word[1] = 0u;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) word |= int4_code(x[i], b, s) << (4 * i);
+                for (int i = 0; i < 16; ++i) word[i / 8] |= int4_code(x[i], b, s) << (4 * (i % 8));
             }
-            *reinterpret_cast<uint32_t*>(dst + (int64_t)off_in * (D / 2) + sub * 4) = word;
+            *reinterpret_cast<uint2*>(dst + (int64_t)off_in * (D / 2) + sub * 8) = make_uint2(word[0], word[1]);
         }
         if (sub == 0)
             *reinterpret_cast<__half2*>(dst + (int64_t)block_of.d * (D / 2) + (int64_t)off_in * 4) =
@@ -191,7 +216,7 @@ __global__ void __launch_bounds__(256) int4_write_kernel(
 
 // Reading rows back: out[t] = the values of slot t (zeros for a slot outside the pool).
 template <typename T, int D>
-__global__ void __launch_bounds__(256) int4_read_kernel(
+__global__ void __launch_bounds__(256, kInt4ReadBlocks) int4_read_kernel(
     const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc, T* __restrict__ k, T* __restrict__ v,
     int64_t first_token, int64_t tokens, int kv_heads, FastDiv rows_of, FastDiv block_of, int64_t page_bytes,
     SlotRows map) {
@@ -202,7 +227,7 @@ __global__ void __launch_bounds__(256) int4_read_kernel(
     if (sub * 8 >= D) return;
     const uint32_t units = (uint32_t)(tokens * kv_heads * 2);
     const uint32_t groups = gridDim.x * (blockDim.x / LPR);
-#pragma unroll 2
+#pragma unroll 4
     for (uint32_t u = blockIdx.x * (blockDim.x / LPR) + threadIdx.x / LPR; u < units; u += groups) {
         const uint32_t t = rows_of(u);
         const uint32_t rest = u - t * rows_of.d, h = rest >> 1;
@@ -226,9 +251,9 @@ __global__ void __launch_bounds__(256) int4_read_kernel(
     }
 }
 
-// Blocks of 256 threads for `units` rows of `lanes` lanes each, at most 8 a SM.
-inline unsigned int4_grid(int64_t units, int lanes, int sms) {
-    const int64_t per = 256 / lanes, blocks = (units + per - 1) / per, cap = (int64_t)sms * 8;
+// Blocks of 256 threads for `units` rows of `lanes` lanes each, at most those that run at once.
+inline unsigned int4_grid(int64_t units, int lanes, int blocks_a_sm, int sms) {
+    const int64_t per = 256 / lanes, blocks = (units + per - 1) / per, cap = (int64_t)sms * blocks_a_sm;
     return (unsigned)(blocks < 1 ? 1 : blocks < cap ? blocks : cap);
 }
 
@@ -244,8 +269,8 @@ static cudaError_t launch_int4_write(void* kc, void* vc, const void* k, const vo
     for (int64_t t = 0; t < tokens && err == cudaSuccess; t += most) {
         const int64_t n = tokens - t < most ? tokens - t : most;
         err = launch_chained(vec ? int4_write_kernel<T, D, true, Rows> : int4_write_kernel<T, D, false, Rows>,
-                             dim3(int4_grid(n * kv_heads * 2, int4_row_lanes(D), sms)), dim3(256), 0, stream,
-                             static_cast<unsigned char*>(kc), static_cast<unsigned char*>(vc),
+                             dim3(int4_grid(n * kv_heads * 2, int4_row_lanes(D, 16), kInt4WriteBlocks, sms)), dim3(256), 0,
+                             stream, static_cast<unsigned char*>(kc), static_cast<unsigned char*>(vc),
                              static_cast<const T*>(k), static_cast<const T*>(v), t, n, kv_heads,
                              FastDiv((uint32_t)kv_heads * 2), FastDiv((uint32_t)block_size),
                              int4_page_bytes(block_size, D), k_stride, v_stride, map);
@@ -260,7 +285,7 @@ static cudaError_t launch_int4_read(const void* kc, const void* vc, void* k, voi
     cudaError_t err = cudaSuccess;
     for (int64_t t = 0; t < tokens && err == cudaSuccess; t += most) {
         const int64_t n = tokens - t < most ? tokens - t : most;
-        err = launch_chained(int4_read_kernel<T, D>, dim3(int4_grid(n * kv_heads * 2, int4_row_lanes(D), sms)),
+        err = launch_chained(int4_read_kernel<T, D>, dim3(int4_grid(n * kv_heads * 2, int4_row_lanes(D), kInt4ReadBlocks, sms)),
                              dim3(256), 0, stream, static_cast<const unsigned char*>(kc),
                              static_cast<const unsigned char*>(vc), static_cast<T*>(k), static_cast<T*>(v), t, n,
                              kv_heads, FastDiv((uint32_t)kv_heads * 2), FastDiv((uint32_t)block_size),

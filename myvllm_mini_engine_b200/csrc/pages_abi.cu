@@ -478,8 +478,8 @@ int minikv_select_blocks(const void* query, const void* bounds, const int64_t* b
     cudaError_t err = cudaSuccess;
     if (table_width > max_blocks) {  // else every request takes all of its blocks
         const int64_t head_groups = (kv_heads + kScoreHeads - 1) / kScoreHeads;
-        // as many spans as two CTAs a SM (their registers) hold at once, each of whole turns of 8 warps
-        const int64_t spans = std::max<int64_t>(1, 2 * sm_count() / (batch * head_groups));
+        // as many spans as two CTAs a SM (one from 192 dims) hold at once, each of whole turns of 8 warps
+        const int64_t spans = std::max<int64_t>(1, (head_dim <= 128 ? 2 : 1) * sm_count() / (batch * head_groups));
         const int64_t span = std::min<int64_t>(kScoreSpan, ((table_width + spans - 1) / spans + 7) / 8 * 8);
         p.span = (int)span;
         const dim3 grid((unsigned)(batch * ((table_width + span - 1) / span)), (unsigned)head_groups);
