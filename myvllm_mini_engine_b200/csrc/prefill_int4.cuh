@@ -45,15 +45,18 @@ constexpr int kPrefillRows = kPrefillWarps * 16;
 constexpr int kPrefillStages = 3;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 2 : 1) prefill_int4_kernel(const PrefillInt4Params p) {
+__global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int4_kernel(const PrefillInt4Params p) {
     constexpr int BN = D <= 128 ? 64 : 32;  // keys a tile: the accumulators of S take BN / 2 registers
     constexpr int RB = D / 2, CPR = RB / 16, NW = D / 32, NT = BN / 8;
     constexpr int STAGE = BN * (2 * RB + 8);  // K codes, V codes, K pairs, V pairs
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     __shared__ __align__(128) unsigned char ring[kPrefillStages * STAGE];
     __shared__ int64_t row_at[2][BN];     // byte of a key's codes in the pool, or -1
     __shared__ int64_t pair_at[2][BN];
     __shared__ uint32_t valid_s[kPrefillStages][2];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
+    // of the keys of a tile, by each warp for itself: K step 2^24, K base, V step, V base
+    __shared__ float4 factors_s[kPrefillWarps][BN];
+    float4* factors = factors_s[warp];
     const int kvh = blockIdx.x, r = blockIdx.z;
     griddep_wait();
     griddep_launch_dependents();
@@ -217,84 +220,101 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 2 : 1) prefill_int
             const unsigned char* st = ring + (kt % kPrefillStages) * STAGE;
             const uint64_t valid = valid_s[kt % kPrefillStages][0] |
                                    (BN > 32 ? (uint64_t)valid_s[kt % kPrefillStages][1] << 32 : 0ull);
-            const __half2* kp = reinterpret_cast<const __half2*>(st + 2 * BN * RB);
-            const __half2* vp = kp + BN;
-            // ---- S: column c of key group j is its key c / 2 + 4 (c % 2)
-            float s[NT][4];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const unsigned char* src = st + (8 * j + (g >> 1) + 4 * (g & 1)) * RB + q4 * (RB / 4);
-                uint32_t w[NW];
-                if constexpr (NW % 4 == 0) {
-#pragma unroll
-                    for (int i = 0; i < NW / 4; ++i) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(src + 16 * i);
-                        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NW; ++i) w[i] = *reinterpret_cast<const uint32_t*>(src + 4 * i);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
-#pragma unroll
-                for (int i = 0; i < NW; ++i) {
-                    mma16816<__half>(s[j], qa[2 * i], w[i] & kNibbleMask, (w[i] >> 8) & kNibbleMask);
-                    mma16816<__half>(s[j], qa[2 * i + 1], w[i] & (kNibbleMask << 4),
-                                     (w[i] >> 8) & (kNibbleMask << 4));
-                }
-            }
-            const bool edge = odd_rows || (kt + 1) * BN > warp_near || valid != (BN == 64 ? ~0ull : 0xffffffffull);
+            const __half2* pairs = reinterpret_cast<const __half2*>(st + 2 * BN * RB);
             float vmax = 0.f;
-            float mx[2] = {-INFINITY, -INFINITY};
-            float vs[NT][2], vb[NT][2];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const int key = 8 * j + q4 + 4 * y;
-                    const float2 a = __half22float2(kp[key]), b = __half22float2(vp[key]);
-                    const float ks = fmaxf(a.x, kInt4StepMin) * kCodeScale;
-                    vs[j][y] = fmaxf(b.x, kInt4StepMin);
-                    vb[j][y] = b.y;
-                    vmax = fmaxf(vmax, vs[j][y]);
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float& e = s[j][2 * x + y];
-                        e = fmaf(e, ks, a.y * qsum[x]);
-                        if (edge && (kt * BN + key > last[x] || !((valid >> key) & 1ull))) e = -INFINITY;
-                        mx[x] = fmaxf(mx[x], e);
-                    }
-                }
+            for (int i = 0; i < BN / 32; ++i) {
+                const float2 k = __half22float2(pairs[32 * i + lane]), v = __half22float2(pairs[BN + 32 * i + lane]);
+                const float vstep = fmaxf(v.x, kInt4StepMin);
+                vmax = fmaxf(vmax, vstep);
+                factors[32 * i + lane] = make_float4(fmaxf(k.x, kInt4StepMin) * kCodeScale, k.y, vstep, v.y);
             }
-            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
-            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-            const int ve = (int)(__float_as_uint(vmax) >> 23) - 127;
+            // the largest step's exponent; O's unit is raised when it exceeds the one in use
+            const int ve = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vmax)) >> 23) - 127;
             const int raise = max(0, ve - vexp);
             vexp += raise;
             const float shrink = raise > 100 ? 0.f : __uint_as_float((uint32_t)(127 - raise) << 23);
             const float vinv = __uint_as_float((uint32_t)(127 - vexp - 1) << 23);
-            float alpha[2];
+            __syncwarp();
+            // ---- S: column c of key group j is its key c / 2 + 4 (c % 2)
+            float s[NT][4];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
-                mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-                const float mn = fmaxf(m[x], mx[x] * qscale[x]);
-                alpha[x] = mn == -INFINITY ? 1.f : exp2_fast(m[x] - mn);
-                m[x] = mn;
-                l[x] *= alpha[x];
-                z[x] *= alpha[x];
+            for (int j = 0; j < NT; j += 2) {  // two groups at a time: their MMA chains overlap
+                uint32_t w[2][NW];
+#pragma unroll
+                for (int jj = 0; jj < 2; ++jj) {
+                    const unsigned char* src = st + (8 * (j + jj) + (g >> 1) + 4 * (g & 1)) * RB + q4 * (RB / 4);
+                    if constexpr (NW % 4 == 0) {
+#pragma unroll
+                        for (int i = 0; i < NW / 4; ++i) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(src + 16 * i);
+                            w[jj][4 * i] = v.x; w[jj][4 * i + 1] = v.y; w[jj][4 * i + 2] = v.z; w[jj][4 * i + 3] = v.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NW; ++i) w[jj][i] = *reinterpret_cast<const uint32_t*>(src + 4 * i);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[j + jj][i] = 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+#pragma unroll
+                    for (int jj = 0; jj < 2; ++jj)
+                        mma16816<__half>(s[j + jj], qa[2 * i], w[jj][i] & kNibbleMask, (w[jj][i] >> 8) & kNibbleMask);
+#pragma unroll
+                    for (int jj = 0; jj < 2; ++jj)
+                        mma16816<__half>(s[j + jj], qa[2 * i + 1], w[jj][i] & (kNibbleMask << 4),
+                                         (w[jj][i] >> 8) & (kNibbleMask << 4));
+                }
             }
-            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f || raise != 0)) {
+            // ---- scores and their maxima
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const float2 f = *reinterpret_cast<const float2*>(&factors[8 * j + q4 + 4 * y]);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float& e = s[j][2 * x + y];
+                        e = fmaf(e, f.x, f.y * qsum[x]);
+                    }
+                }
+            if (odd_rows || (kt + 1) * BN > warp_near || valid != (BN == 64 ? ~0ull : 0xffffffffull)) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = 8 * j + q4 + 4 * (i & 1);
+                        if (kt * BN + key > last[i >> 1] || !((valid >> key) & 1ull)) s[j][i] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], s[j][i]);
+            const bool higher = mx[0] * qscale[0] > m[0] + kMaxSlack || mx[1] * qscale[1] > m[1] + kMaxSlack;
+            if (__any_sync(0xffffffffu, higher || raise != 0)) {
+                float alpha[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
+                    mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
+                    const float top = mx[x] * qscale[x];
+                    const float mn = top > m[x] + kMaxSlack ? top : m[x];
+                    alpha[x] = mn == -INFINITY ? 1.f : exp2_fast(m[x] - mn);
+                    m[x] = mn;
+                    l[x] *= alpha[x];
+                    z[x] *= alpha[x];
+                    alpha[x] *= shrink;
+                }
 #pragma unroll
                 for (int u = 0; u < NW; ++u)
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        o[u][n][0] *= alpha[0] * shrink;
-                        o[u][n][1] *= alpha[0] * shrink;
-                        o[u][n][2] *= alpha[1] * shrink;
-                        o[u][n][3] *= alpha[1] * shrink;
-                    }
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[u][n][i] *= alpha[i >> 1];
             }
             // ---- P, and P step' as the A operand; O, 16 keys at a time
             const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
@@ -302,7 +322,13 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 2 : 1) prefill_int
             for (int j = 0; j < NT; j += 2) {
                 uint32_t a[4];
 #pragma unroll
-                for (int jj = 0; jj < 2; ++jj)
+                for (int jj = 0; jj < 2; ++jj) {
+                    float2 f[2];  // V step, V base of the two keys
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        f[y] = *reinterpret_cast<const float2*>(&factors[8 * (j + jj) + q4 + 4 * y].z);
+                        f[y].x *= vinv;
+                    }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         float w[2];
@@ -310,11 +336,12 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 2 : 1) prefill_int
                         for (int y = 0; y < 2; ++y) {
                             const float e = exp2_fast(fmaf(s[j + jj][2 * x + y], qscale[x], -mm[x]));
                             l[x] += e;
-                            z[x] = fmaf(e, vb[j + jj][y], z[x]);
-                            w[y] = e * (vs[j + jj][y] * vinv);
+                            z[x] = fmaf(e, f[y].y, z[x]);
+                            w[y] = e * f[y].x;
                         }
                         a[2 * jj + x] = Elem<__half>::pack(w[0], w[1]);
                     }
+                }
                 const unsigned char* v = st + (BN + 8 * j + q4) * RB + g * (RB / 8);
                 uint32_t x0[NW], x1[NW];
 #pragma unroll
@@ -353,11 +380,13 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 2 : 1) prefill_int
                 }
 #pragma unroll
                 for (int u = 0; u < NW; ++u) {
-                    mma16816<__half>(o[u][0], a, x0[u] & kNibbleMask, x1[u] & kNibbleMask);
-                    mma16816<__half>(o[u][1], a, x0[u] & (kNibbleMask << 4), x1[u] & (kNibbleMask << 4));
-                    mma16816<__half>(o[u][2], a, (x0[u] >> 8) & kNibbleMask, (x1[u] >> 8) & kNibbleMask);
-                    mma16816<__half>(o[u][3], a, (x0[u] >> 8) & (kNibbleMask << 4),
-                                     (x1[u] >> 8) & (kNibbleMask << 4));
+                    // even nibbles, and whole bytes for the odd ones (as the decode)
+                    const uint32_t l0 = x0[u] & 0x00ff00ffu, l1 = x1[u] & 0x00ff00ffu;
+                    const uint32_t h0 = permute_bytes(x0[u], 0u, 0x4341u), h1 = permute_bytes(x1[u], 0u, 0x4341u);
+                    mma16816<__half>(o[u][0], a, l0 & kNibbleMask, l1 & kNibbleMask);
+                    mma16816<__half>(o[u][1], a, l0, l1);
+                    mma16816<__half>(o[u][2], a, h0 & kNibbleMask, h1 & kNibbleMask);
+                    mma16816<__half>(o[u][3], a, h0, h1);
                 }
             }
         }
@@ -380,8 +409,9 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 2 : 1) prefill_int
 #pragma unroll
                 for (int u = 0; u < NW; ++u) {
                     const int i = 2 * x + y;
-                    const float f0 = fmaf(o[u][0][i], up, Z) * inv, f1 = fmaf(o[u][1][i], up * 0.0625f, Z) * inv;
-                    const float f2 = fmaf(o[u][2][i], up, Z) * inv, f3 = fmaf(o[u][3][i], up * 0.0625f, Z) * inv;
+                    const float f0 = fmaf(o[u][0][i], up, Z) * inv, f2 = fmaf(o[u][2][i], up, Z) * inv;
+                    const float f1 = fmaf(o[u][1][i] - o[u][0][i], up * 0.0625f, Z) * inv;
+                    const float f3 = fmaf(o[u][3][i] - o[u][2][i], up * 0.0625f, Z) * inv;
                     *reinterpret_cast<uint2*>(dst + 4 * u) = make_uint2(Elem<T>::pack(f0, f1), Elem<T>::pack(f2, f3));
                 }
             }
