@@ -345,13 +345,22 @@ int minikv_paged_decode_int4(const void* query, const void* key_cache, const voi
                              int64_t block_size, int64_t table_width, int64_t max_blocks, int dtype, void* stream);
 
 /* Ragged causal prefill over a 4-bit pool: minikv_paged_prefill's contract with
- * an fp16/bf16 query and output and up to 64 query heads a kv head; no
- * workspace.  Tokens of no request, or past their context, get zero rows. */
+ * an fp16/bf16 query and output and up to 64 query heads a kv head.  Tokens of
+ * no request, or past their context, get zero rows.  Two routes: the codes as
+ * operands, exact, for every shape; and, for bf16 batches of enough queries a
+ * request on the tcgen05 prefill's shapes, that kernel on an fp16 copy of the
+ * pages the tables reference (base + step * code rounded to fp16, Q saturated to
+ * fp16's range), made in the workspace (256-byte aligned; 0 bytes on the other
+ * route, where none is read). */
+int64_t minikv_paged_prefill_int4_workspace_bytes(int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
+                                                  int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                                                  int64_t table_width, int dtype);
 int minikv_paged_prefill_int4(const void* q, const void* key_cache, const void* value_cache,
                               const int64_t* cu_seqlens_q, const int64_t* query_starts, const int64_t* block_tables,
-                              const int64_t* context_lens, void* out, int64_t tokens, int64_t requests,
-                              int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks,
-                              int64_t block_size, int64_t table_width, int64_t max_query_len, int dtype, void* stream);
+                              const int64_t* context_lens, void* out, void* workspace, int64_t workspace_bytes,
+                              int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                              int64_t num_blocks, int64_t block_size, int64_t table_width, int64_t max_query_len,
+                              int dtype, void* stream);
 
 /* ---------------------------------------------------------- block selection ---
  * No counterpart in the reference.  Attention that reads, for each request and

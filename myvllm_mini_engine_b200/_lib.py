@@ -55,7 +55,8 @@ SIGNATURES = {
     "minikv_kv_gather_slots_int4": (_int, [_p] * 5 + [_i64] * 5 + [_int, _p]),
     "minikv_paged_decode_int4_workspace_bytes": (_i64, [_i64] * 7 + [_int]),
     "minikv_paged_decode_int4": (_int, [_p] * 9 + [_i64] + [_i64] * 8 + [_int, _p]),
-    "minikv_paged_prefill_int4": (_int, [_p] * 8 + [_i64] * 9 + [_int, _p]),
+    "minikv_paged_prefill_int4_workspace_bytes": (_i64, [_i64] * 8 + [_int]),
+    "minikv_paged_prefill_int4": (_int, [_p] * 9 + [_i64] * 10 + [_int, _p]),
     "minikv_block_bounds_update": (_int, [_p] * 5 + [_i64] * 7 + [_int, _p]),
     "minikv_block_bounds_read": (_int, [_p, _p, _i64, _p, _p] + [_i64] * 3 + [_p]),
     "minikv_select_blocks_workspace_bytes": (_i64, [_i64] * 3),

@@ -6,6 +6,8 @@ Writes match the oracle byte for byte.  Attention: with V values in a range of
   spread * (2^-12 P' rounded to fp16 once, as bf16 outputs and the prefill have it; 2^-22 in two
   terms) plus spread * 2 ln 2 * ds for scores off by ds (log2), where an fp32 dot product of D
   terms is off by at most (D + 8) 2^-23 of the sum of its terms' magnitudes.
+The bf16 prefill over an fp16 copy of the pages: half a step of fp16, 2^-11, of every K (in ds, of the
+sum of the products' magnitudes) and V besides.
 """
 
 import math
@@ -42,20 +44,24 @@ def tables_for(gen, lens, block_size, spare=3):
     return table, blocks
 
 
-def assert_near(actual, expected, query, keys, vals, dtype, one_term):
+def assert_near(actual, expected, query, keys, vals, dtype, one_term, copied=False):
     """The bound of the module's docstring, element by element, and half a step of the type over the whole."""
     finite_k, finite_v = keys[torch.isfinite(keys)], vals[torch.isfinite(vals)]
     spread = float(finite_v.max() - finite_v.min())
     dim = query.shape[-1]
     terms = float(query.double().abs().sum(-1).max()) * float(finite_k.abs().max()) * 2  # codes and base apart
     ds = (dim + 8) * 2.0 ** -23 * terms * math.log2(math.e) / math.sqrt(dim)
-    inner = spread * ((2.0 ** -12 if one_term else 2.0 ** -22) + 2 * math.log(2) * ds)
+    copy = 2.0 ** -11 * float(finite_v.abs().max()) if copied else 0.0
+    if copied:
+        ds += 2.0 ** -11 * terms / 2 * math.log2(math.e) / math.sqrt(dim)
+    inner = spread * ((2.0 ** -12 if one_term else 2.0 ** -22) + 2 * math.log(2) * ds) + copy
     half = torch.finfo(dtype).eps / 2
     err = (actual.double().cpu() - expected).abs()
     assert bool((err <= half * expected.abs() + inner + 2.0 ** -25).all()), float(err.max())
     norm = float(expected.norm())
-    if norm:
-        assert float((actual.double().cpu() - expected).norm()) <= (half + 2.0 ** -11) * norm
+    if norm:  # (below 2^-14 an fp16's half step is 2^-25, whatever the value)
+        least = 2.0 ** -25 * math.sqrt(expected.numel()) if dtype == torch.float16 else 0.0
+        assert float((actual.double().cpu() - expected).norm()) <= (half + 2.0 ** -11) * norm + least
 
 
 def decode(gen, dtype, lens, heads, kv_heads, dim, block_size, *, tables=None, scale=1.0, selected=None,
@@ -335,7 +341,10 @@ def prefill(gen, dtype, counts, starts, heads, kv_heads, dim, block_size, *, tab
                                           starts.cuda(), table.cuda(), lens.cuda(), block_size, validate=validate,
                                           max_query_len=max_query_len)
     assert actual.dtype == dtype and actual.shape == q.shape
-    assert_near(actual, expected, q, keys, vals, dtype, True)
+    # the rule of the two routes: bf16, head_dim 64 or 128, enough rows a request, the tcgen05 kernel's pages
+    copied = (dtype == torch.bfloat16 and dim in (64, 128) and block_size % 8 == 0 and 128 % (heads // kv_heads) == 0
+              and q.shape[0] * (heads // kv_heads) >= 128 * len(counts))
+    assert_near(actual, expected, q, keys, vals, dtype, True, copied)
     return actual
 
 
@@ -361,7 +370,8 @@ def test_prefill_extreme_scales(cuda_device, scale):
     prefill(np.random.default_rng(21), torch.bfloat16, (50,), (90,), 4, 2, 64, 16, scale=scale)
 
 
-def test_prefill_growing_steps(cuda_device):
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prefill_growing_steps(cuda_device, dtype):
     """Values whose steps grow along the keys by far more than fp16's range."""
     gen = np.random.default_rng(22)
     bs, dim, n = 16, 64, 400
@@ -370,7 +380,7 @@ def test_prefill_growing_steps(cuda_device):
     int4_kv.scatter(kp, bs, torch.arange(n), randn(gen, n, 1, dim))
     int4_kv.scatter(vp, bs, torch.arange(n), v)
     keys, vals = int4_kv.values(kp, bs, dim), int4_kv.values(vp, bs, dim)
-    q = randn(gen, n, 2, dim).to(torch.bfloat16)
+    q = randn(gen, n, 2, dim).to(dtype)
     cu, starts, lens = torch.tensor([0, n]), torch.tensor([0]), torch.tensor([n])
     table = torch.arange(25).view(1, 25)
     expected = int4_kv.paged_prefill(q, keys, vals, cu, starts, table, lens, bs)
@@ -379,21 +389,63 @@ def test_prefill_growing_steps(cuda_device):
     # row by row: each has its own range of values (those it sees)
     for i in range(0, n, 7):
         assert_near(actual[i:i + 1], expected[i:i + 1], q[i:i + 1], keys, vals.view(-1, 1, dim)[:i + 1],
-                    torch.bfloat16, True)
+                    dtype, True, dtype == torch.bfloat16)
 
 
-def test_prefill_guards(cuda_device):
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("more", [0, 100])
+def test_prefill_guards(cuda_device, dtype, more):
     """Invalid pages, contexts that end early, tokens of no request, a bound below a request's length."""
     def spoil(table):
         table[0, 1] = -1
         table[1].fill_(1 << 33)
         return table
 
-    actual = prefill(np.random.default_rng(23), torch.bfloat16, (60, 20, 50), (0, 7, 30), 4, 2, 64, 16, tables=spoil,
-                     lens=(60, 27, 60), extra=9, validate=False, max_query_len=10)
+    first = 60 + more  # long chunks take the other route of bf16
+    actual = prefill(np.random.default_rng(23), dtype, (first, 20, 50), (0, 7, 30), 4, 2, 64, 16, tables=spoil,
+                     lens=(first, 27, 60), extra=9, validate=False, max_query_len=200 if more else 10)
+    actual = actual[more:]
     assert not actual[60:80].any()          # every page of request 1 is invalid
     assert not actual[110:130].any()        # positions 60..79 of request 2 lie past its context
     assert not actual[130:].any()           # tokens of no request
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads,block_size,counts,starts", [
+    (128, 8, 4, 16, (200, 64, 130), (37, 0, 500)), (64, 4, 4, 8, (300, 1), (5, 700)), (128, 16, 1, 24, (20, 9), (0, 90)),
+    (64, 32, 1, 256, (33,), (255,)), (128, 2, 2, 64, (128, 128), (0, 0))])
+def test_prefill_over_a_copy(cuda_device, dim, heads, kv_heads, block_size, counts, starts):
+    """bf16 batches of enough queries a request, on the tcgen05 prefill."""
+    prefill(np.random.default_rng(dim + heads), torch.bfloat16, counts, starts, heads, kv_heads, dim, block_size)
+
+
+def test_prefill_in_a_graph(cuda_device):
+    """Both routes, captured with one split of the queries and replayed with another."""
+    gen = np.random.default_rng(25)
+    table, blocks = tables_for(gen, [400, 400], 16)
+    kp, vp = make_pool(gen, blocks, 16, 2, 64), make_pool(gen, blocks, 16, 2, 64)
+    keys, vals = int4_kv.values(kp, 16, 64), int4_kv.values(vp, 16, 64)
+    kp, vp, gpu_table = torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(), table.cuda()
+    for dtype in (torch.float16, torch.bfloat16):
+        q = randn(gen, 200, 4, 64).to(dtype)
+        cu, starts, lens = torch.tensor([0, 120, 200]), torch.tensor([10, 20]), torch.tensor([130, 100])
+        gpu = [x.cuda() for x in (q, cu, starts, lens)]
+        run = lambda: paged_prefill_attention_int4(gpu[0], kp, vp, gpu[1], gpu[2], gpu_table, gpu[3], 16,  # noqa: E731
+                                                   validate=False)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        cu, starts, lens = torch.tensor([0, 50, 200]), torch.tensor([300, 0]), torch.tensor([350, 150])
+        for held, new in zip(gpu[1:], (cu, starts, lens)):
+            held.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        expected = int4_kv.paged_prefill(q, keys, vals, cu, starts, table, lens, 16)
+        assert_near(out, expected, q, keys, vals, dtype, True, dtype == torch.bfloat16)
 
 
 def test_prefill_matches_decode(cuda_device):

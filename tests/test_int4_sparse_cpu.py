@@ -158,12 +158,12 @@ def test_c_entry_points_refuse():
     for rc in (lib.minikv_kv_scatter_slots_int4(*[None] * 5, 0, 8, 16, 2, 64, 128, 128, _lib.BF16, None),
                lib.minikv_kv_append_batch_int4(*[None] * 6, 0, 2, 8, 16, 2, 64, 128, 128, _lib.BF16, None),
                lib.minikv_kv_gather_slots_int4(*[None] * 5, 0, 8, 16, 2, 64, _lib.BF16, None),
-               lib.minikv_paged_prefill_int4(*[None] * 8, 0, 1, 4, 2, 64, 8, 16, 4, 1, _lib.BF16, None),
+               lib.minikv_paged_prefill_int4(*[None] * 9, 0, 0, 1, 4, 2, 64, 8, 16, 4, 1, _lib.BF16, None),
                lib.minikv_block_bounds_update(*[None] * 5, 0, 4, 8, 16, 2, 64, 1, _lib.BF16, None),
                lib.minikv_block_bounds_read(None, None, 0, None, None, 8, 2, 64, None)):
         assert rc == _lib.OK  # empty calls touch nothing
-    refused(lib.minikv_paged_prefill_int4(*[p] * 8, 5, 70000, 4, 2, 64, 8, 16, 4, 1, _lib.BF16, None), "requests")
-    assert lib.minikv_paged_prefill_int4(*[p] * 8, 5, 1, 65, 1, 64, 8, 16, 4, 1, _lib.BF16, None) == _lib.EUNSUPPORTED
+    refused(lib.minikv_paged_prefill_int4(*[p] * 9, 0, 5, 70000, 4, 2, 64, 8, 16, 4, 1, _lib.BF16, None), "requests")
+    assert lib.minikv_paged_prefill_int4(*[p] * 9, 0, 5, 1, 65, 1, 64, 8, 16, 4, 1, _lib.BF16, None) == _lib.EUNSUPPORTED
     refused(lib.minikv_block_bounds_update(*[p] * 5, 1, 4, 8, 16, 2, 64, 1, 7, None), "4-bit")
     select = [p] * 6 + [1 << 20]
     refused(lib.minikv_select_blocks(*select, 2, 8, 4, 64, 10, 16, 4, 3, 2, 2, _lib.BF16, None), "max_blocks")
