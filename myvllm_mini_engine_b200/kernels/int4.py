@@ -77,9 +77,18 @@ def _source_rows(tensor):
     return tensor.contiguous(), heads * dim
 
 
+def _extent(tensor):
+    """(first byte, byte behind the last) of a tensor's elements."""
+    last = sum((n - 1) * stride for n, stride in zip(tensor.shape, tensor.stride()))
+    start = tensor.data_ptr()
+    return start, start + (last + 1) * tensor.element_size() if tensor.numel() else start
+
+
 def _overlaps(caches, sources):
-    return (torch._C._overlaps(*caches)
-            or any(torch._C._overlaps(cache, source) for cache in caches for source in sources))
+    """Whether a cache shares bytes with the other one or with a source (views of one storage need not)."""
+    held = [_extent(cache) for cache in caches]
+    ranges = [*held[1:], *map(_extent, sources)]
+    return any(a < d and c < b for i, (a, b) in enumerate(held) for c, d in ranges[i:])
 
 
 def write_kv_cache_slots_int4(key_cache, value_cache, slot_mapping, key, value, block_size, *, backend="cuda",
