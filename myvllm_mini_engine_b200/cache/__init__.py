@@ -1,4 +1,4 @@
 from .cow import copy_on_write, prepare_write
-from .kv_cache import FP8KVCachePool, PagedKVPool, PoolShape
+from .kv_cache import FP8KVCachePool, INT4KVCachePool, PagedKVPool, PoolShape
 
-__all__ = ["FP8KVCachePool", "PagedKVPool", "PoolShape", "copy_on_write", "prepare_write"]
+__all__ = ["FP8KVCachePool", "INT4KVCachePool", "PagedKVPool", "PoolShape", "copy_on_write", "prepare_write"]

@@ -50,9 +50,11 @@ import torch
 from torch.nn import functional as F
 
 from .. import _lib
-from ..cache.kv_cache import FP8KVCachePool, PagedKVPool
+from ..cache.kv_cache import FP8KVCachePool, INT4KVCachePool, PagedKVPool
+from ..kernels.data import write_kv_cache_batch
 from ..kernels.fp8 import paged_attention_fp8_with_append
 from ..kernels.paged import paged_attention_with_append
+from ..kernels.sparse import paged_attention_selected
 
 
 @dataclass(frozen=True)
@@ -208,7 +210,14 @@ class Qwen3DecodeStep:
     head_dim) in the weights' dtype and device, or an :class:`FP8KVCachePool`
     (an extension: the new token's K/V are written by the same kernels into a
     small bf16 staging buffer, then quantised into the pool by the FP8 slot
-    scatter, and the attention reads the FP8 pool).  ``forward_decode_batch``
+    scatter, and the attention reads the FP8 pool), or an
+    :class:`INT4KVCachePool` (its rows quantised from the staging buffer by the
+    4-bit append).  With ``selected_blocks`` the attention of every layer reads
+    only that many blocks a request and kv head, chosen by the layer's query from
+    the pool's block bounds (a 16-bit or 4-bit pool made with
+    ``block_bounds=True``, whose history's bounds are up to date; the step updates
+    those of the rows it appends); requests of no more blocks are attended whole.
+    ``forward_decode_batch``
     follows ``NativeQwen3.forward_decode_batch`` (native_qwen3.py:423-456):
     it returns the logits ``[B, vocab]`` and appends each request's new K/V at
     ``positions[b]`` through ``block_tables[b]``.
@@ -218,14 +227,19 @@ class Qwen3DecodeStep:
     FUSED_MAX_BATCH = 32
 
     def __init__(self, config: Qwen3Config, weights: Qwen3Weights, pool: PagedKVPool, *,
-                 fused_projections: bool | None = None):
+                 fused_projections: bool | None = None, selected_blocks: int | None = None):
         shape = pool.shape
         if (shape.num_layers, shape.num_kv_heads, shape.head_dim) != (
                 config.num_hidden_layers, config.num_key_value_heads, config.head_dim):
             raise ValueError("KV cache architecture mismatch")
         self.fp8 = isinstance(pool, FP8KVCachePool)
-        if pool.key.device != weights.embed.device or (not self.fp8 and pool.dtype != weights.embed.dtype):
+        self.int4 = isinstance(pool, INT4KVCachePool)
+        if pool.key.device != weights.embed.device or (not self.fp8 and not self.int4
+                                                       and pool.dtype != weights.embed.dtype):
             raise ValueError("cache must match model device and dtype")
+        if selected_blocks is not None and (selected_blocks < 2 or getattr(pool, "bounds", None) is None):
+            raise ValueError("selected_blocks needs 2 blocks or more and a pool with block bounds")
+        self.selected_blocks = selected_blocks
         if weights.embed.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError("the decode step runs in FP16/BF16")
         if config.head_dim not in (64, 128, 256):
@@ -403,6 +417,8 @@ class Qwen3DecodeStep:
         batch = q.shape[0]
         rows = (batch, self.config.num_key_value_heads, self.config.head_dim)
         stage_k, stage_v = self._stage_k.view(rows), self._stage_v.view(rows)
+        if self.int4 or self.selected_blocks is not None:
+            return self._attend_pages(index, q, block_tables, positions, stage_k, stage_v)
         if not self.fp8:
             return paged_attention_with_append(q, pool.key[index], pool.value[index], block_tables, positions,
                                                stage_k, stage_v, pool.shape.block_size, validate=False,
@@ -410,6 +426,23 @@ class Qwen3DecodeStep:
         return paged_attention_fp8_with_append(q, pool.key[index], pool.value[index], block_tables, positions,
                                                stage_k, stage_v, pool.shape.block_size, pool.k_scale, pool.v_scale,
                                                kv_format=pool.kv_format, validate=False, chained=True)
+
+    def _attend_pages(self, index, q, block_tables, positions, stage_k, stage_v):
+        """Append, then attend a 4-bit pool, or the blocks selected from the pool's bounds."""
+        pool, lengths = self.pool, positions + 1
+        if self.int4:
+            pool.write_batch(index, block_tables, positions, stage_k, stage_v, validate=False)
+        else:
+            write_kv_cache_batch(pool.key[index], pool.value[index], block_tables, positions, stage_k, stage_v,
+                                 pool.shape.block_size, validate=False)
+        selected = None
+        if self.selected_blocks is not None:
+            pool.update_bounds(index, block_tables, positions, lengths, validate=False, max_query_len=1)
+            selected = pool.select_blocks(index, q, block_tables, lengths, self.selected_blocks, validate=False)
+        if self.int4:
+            return pool.attend(index, q, block_tables, lengths, selected=selected, validate=False)
+        return paged_attention_selected(q, pool.key[index], pool.value[index], block_tables, lengths, selected,
+                                        pool.shape.block_size, validate=False)
 
     def greedy(self, input_ids, block_tables, positions):
         """Greedy next token of every request (argmax of the step's logits)."""

@@ -196,3 +196,61 @@ def test_oracle_scores_bound_the_products():
     assert bound >= float((keys @ query.double().T).sum(1).max()) - 1e-5
     codes = block_select.query_codes(query)
     assert codes.shape == (128,) and int(np.abs(codes).max()) == 127
+
+
+def test_overlap_is_of_bytes_not_of_storages():
+    from myvllm_mini_engine_b200.kernels.int4 import _overlaps
+
+    both = torch.zeros(2, 64, dtype=torch.uint8)
+    other = torch.zeros(4, 2, 8, dtype=torch.bfloat16)
+    assert not _overlaps((both[0], both[1]), (other, other[:, 1]))
+    assert _overlaps((both[0], both.view(-1)[63:]), (other,))
+    assert not _overlaps((both[0], both[1]), (both[1, :0],))
+    halves = torch.zeros(4, 2, 8, dtype=torch.bfloat16).view(torch.uint8)
+    for i in range(2):  # a source that lies in either cache, strided too
+        caches = [both[0], both[1]]
+        caches[i] = halves.view(-1)[:64]
+        assert _overlaps(caches, (halves.view(torch.bfloat16)[1:, 1],))
+
+
+def test_pools_check_their_arguments():
+    from myvllm_mini_engine_b200.cache import INT4KVCachePool, PagedKVPool
+
+    with pytest.raises(ValueError, match="head_dim"):
+        INT4KVCachePool(1, 4, 16, 2, 80, device="cpu")
+    with pytest.raises(ValueError, match="positive"):
+        INT4KVCachePool(1, 0, 16, 2, 64, device="cpu")
+    pool = INT4KVCachePool(2, 4, 16, 2, 64, device="cpu")
+    assert pool.memory_bytes == 2 * 2 * 4 * 2 * 16 * 36 and pool.bounds is None
+    one = torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(ValueError, match="block bounds"):
+        pool.update_bounds(0, one[None], one, one)
+    with pytest.raises(IndexError, match="layer"):
+        pool.write_range(2, [0], 0, rows(), rows())
+    with pytest.raises(IndexError, match="block id"):
+        pool.write_range(0, [7], 0, rows(), rows())
+    with pytest.raises(ValueError, match="capacity"):
+        pool.write_range(0, [0], 15, rows(), rows())
+    with pytest.raises(ValueError, match="CUDA"):  # no CPU path
+        pool.write_slots(0, torch.arange(3), rows(), rows())
+    with pytest.raises(ValueError, match="16-bit and 4-bit"):
+        PagedKVPool(1, 4, 16, 2, 64, dtype=torch.float32, device="cpu", block_bounds=True)
+    with pytest.raises(ValueError, match="head_dim"):
+        PagedKVPool(1, 4, 16, 2, 80, device="cpu", block_bounds=True)
+    held = PagedKVPool(3, 4, 16, 2, 64, device="cpu", block_bounds=True)
+    assert held.bounds.shape == (3, 4, 2, k.block_bounds_bytes(64))
+
+
+def test_decode_step_checks_its_pool():
+    from myvllm_mini_engine_b200.cache import FP8KVCachePool, INT4KVCachePool, PagedKVPool
+    from myvllm_mini_engine_b200.engine.qwen3 import Qwen3Config, Qwen3DecodeStep, Qwen3Weights
+
+    cfg = Qwen3Config.qwen3_0_6b(num_hidden_layers=1, vocab_size=64)
+    weights = Qwen3Weights.random(cfg, dtype=torch.bfloat16, device="cpu", seed=0)
+    shape = (1, 4, 16, cfg.num_key_value_heads, cfg.head_dim)
+    for pool in (PagedKVPool(*shape, device="cpu"), INT4KVCachePool(*shape, device="cpu"),
+                 FP8KVCachePool(*shape, k_scale=1.0, v_scale=1.0, device="cpu")):
+        with pytest.raises(ValueError, match="block bounds"):
+            Qwen3DecodeStep(cfg, weights, pool, selected_blocks=4)
+    with pytest.raises(ValueError, match="2 blocks"):
+        Qwen3DecodeStep(cfg, weights, INT4KVCachePool(*shape, device="cpu", block_bounds=True), selected_blocks=1)
