@@ -24,11 +24,15 @@
 // a fixed order.  A unit that spans CTAs leaves one partial per CTA; the CTA
 // that takes the unit's last ticket joins them, in the order of the CTAs.
 //
-// Bound by the bytes of the pages.  TMA boxes or bulk copies of a page's head
-// (1 KB at D = 128, block_size 16) would hit the SM's copy rate of about one per
-// 45 ns, 3.4 TB/s over the device, so the copies are per lane.  mma.sync rather
-// than tcgen05: the group's few query heads are the N = 8 columns, the operands
-// are made in registers, and the tensor pipe is far from its limit.
+// Long batches are bound by the instructions that make the operands: about 580
+// a tile of 32 tokens at D = 128, of the 760 that the SM issues in the time that
+// its share of the memory's rate brings the tile (256 requests of 4096 tokens, 8
+// kv heads: 235 us, 4.9 TB/s of the pool, against 177 us at the measured copy
+// rate); small ones by the chain of launch, look-ups, pages and join (8 x 513:
+// 12 us).  Copies a lane rather than bulk copies of a page's head (1 KB at D =
+// 128, block_size 16): both reach the memory's rate here, and these need no
+// barrier and no producer.  mma.sync rather than tcgen05: the group's few query
+// heads are the N = 8 columns, and the operands are made in registers.
 #pragma once
 
 #include "common.cuh"
@@ -686,7 +690,7 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 
     const int64_t team = alone ? (int64_t)blockIdx.x * W + warp : blockIdx.x;
     int64_t G = (int64_t)gridDim.x * (alone ? W : 1);  // runs
     // Every run has a tile, of a CTA at least one for each warp; where that is no more than four a warp,
-    // a whole unit's, which then needs no join (8 x 513 tokens: 17.8 -> TIMING us).
+    // a whole unit's, which then needs no join (8 x 513 tokens: 17.8 -> 12.3 us).
     const int least = longest <= 4 * W ? max(W, longest) : W;
     G = min(G, alone ? total : (total + least - 1) / least);
     if (team >= G) return;

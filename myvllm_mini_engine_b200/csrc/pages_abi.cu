@@ -141,6 +141,15 @@ int check_decode(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_
     return MINIKV_OK;
 }
 
+// Tiles of 16 tokens: a request's, those of all requests of one head, and a run's are counted in 31 bits.
+int check_tiles(int64_t batch, int64_t q_heads, int64_t block_size, int64_t width) {
+    const int64_t tiles = width * block_size / 16 + 1;
+    PAGES_REQUIRE(tiles <= 2147483647 / batch && tiles <= 2147483647 / q_heads &&
+                      batch * tiles <= (1ll << 37) / q_heads,
+                  MINIKV_EINVAL, "batch, heads and table capacity together are too large");
+    return MINIKV_OK;
+}
+
 // Calls f with the consumer type and whether the pool is 4-bit.
 template <typename F> auto with_consumer(bool int4, int dtype, int64_t dim, F f) {
     return with_type16(dtype, [&](auto t) {
@@ -177,8 +186,8 @@ int run_page_decode(bool int4, const void* query, const void* key_cache, const v
                     unsigned int* tickets, void* workspace, int64_t workspace_bytes, int64_t batch, int64_t q_heads,
                     int64_t kv_heads, int64_t dim, int64_t num_blocks, int64_t block_size, int64_t width,
                     int64_t take, int dtype, void* stream) {
-    const int rc = check_decode(batch, q_heads, kv_heads, dim, num_blocks, block_size, width, take,
-                                selected != nullptr, dtype);
+    int rc = check_decode(batch, q_heads, kv_heads, dim, num_blocks, block_size, width, take, selected != nullptr, dtype);
+    if (rc == MINIKV_OK) rc = check_tiles(batch, q_heads, block_size, width);
     if (rc) return rc;
     PAGES_REQUIRE(query && key_cache && value_cache && tables && lens && out, MINIKV_EINVAL, "null pointer argument");
     PAGES_REQUIRE(aligned16(query) && aligned16(key_cache) && aligned16(value_cache) && aligned16(out), MINIKV_EINVAL,
@@ -308,7 +317,8 @@ int minikv_kv_gather_slots_int4(const void* key_cache, const void* value_cache, 
 int64_t minikv_paged_decode_int4_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                                  int64_t num_blocks, int64_t block_size, int64_t table_width,
                                                  int dtype) {
-    if (check_decode(batch, q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, 1, false, dtype))
+    if (check_decode(batch, q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, 1, false, dtype) ||
+        check_tiles(batch, q_heads, block_size, table_width))
         return -1;
     PageDecodePlan plan;
     decode_plan(true, batch, q_heads, kv_heads, head_dim, dtype, &plan);
@@ -555,7 +565,8 @@ int minikv_select_blocks(const void* query, const void* bounds, const int64_t* b
 int64_t minikv_paged_decode_selected_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                      int64_t head_dim, int64_t num_blocks, int64_t block_size,
                                                      int64_t table_width, int dtype) {
-    if (check_decode(batch, q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, 1, false, dtype))
+    if (check_decode(batch, q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, 1, false, dtype) ||
+        check_tiles(batch, q_heads, block_size, table_width))
         return -1;
     PageDecodePlan plan;
     decode_plan(false, batch, q_heads, kv_heads, head_dim, dtype, &plan);

@@ -55,9 +55,11 @@ def update_block_bounds(bounds, key_cache, block_tables, query_starts, context_l
     head_dim]`` or a 4-bit pool ``[num_blocks, kv_heads, page_bytes]``.  A block's
     bounds cover all of its rows below ``context_lens[r]``.  For a decode step pass
     the new row's position and position + 1.  ``max_query_len`` (optional) bounds
-    ``context_lens - query_starts`` on the host; blocks past it are not updated.
-    Empty ranges update nothing; out-of-range requests and pages are skipped
-    (refused with ``validate``).
+    ``context_lens - query_starts`` on the host; blocks past it are not updated
+    (refused with ``validate``).  Empty ranges update nothing; out-of-range requests
+    and pages are skipped (refused with ``validate``).  A block that several requests
+    name has to hold the same rows for each of them, as full shared blocks do; its
+    bounds would depend on their order else (refused with ``validate``).
     """
     check_backend(backend)
     num_blocks, kv_heads, dim = _check_bounds(bounds)
@@ -95,6 +97,12 @@ def update_block_bounds(bounds, key_cache, block_tables, query_starts, context_l
                   & (query_starts < context_lens)[:, None])
         _require(not bool((((block_tables < 0) | (block_tables >= num_blocks)) & active).any()),
                  "physical block id out of range")
+        _require(max_query_len is None or not bool((context_lens - query_starts > int(max_query_len)).any()),
+                 "max_query_len is below a request's rows")
+        pages = block_tables[active]
+        rows = (context_lens[:, None] - column * block_size).clamp(max=block_size)[active]
+        _require(pages.unique().numel() == (pages * (block_size + 1) + rows).unique().numel(),
+                 "a block of several requests must hold the same rows for each")
     if requests == 0:
         return
     longest = width * block_size if max_query_len is None else int(max_query_len)

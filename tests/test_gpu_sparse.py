@@ -95,6 +95,19 @@ def test_bounds_guards(cuda_device):
     assert np.array_equal(got.cpu().numpy(), want)
 
 
+def test_bounds_refuse_what_depends_on_the_order(cuda_device):
+    keys = torch.randn(4, 16, 2, 64, device="cuda").half()
+    bounds = torch.zeros(4, 2, block_bounds_bytes(64), dtype=torch.uint8, device="cuda")
+    table = torch.tensor([[0, 1], [0, 2]], device="cuda")
+    starts = torch.zeros(2, dtype=torch.int64, device="cuda")
+    update_block_bounds(bounds, keys, table, starts, torch.tensor([20, 32]).cuda(), 16)  # a full shared block
+    with pytest.raises(RuntimeError, match="same rows"):
+        update_block_bounds(bounds, keys, table, starts, torch.tensor([20, 9]).cuda(), 16)
+    update_block_bounds(bounds, keys, table, starts, torch.tensor([20, 16]).cuda(), 16, max_query_len=20)
+    with pytest.raises(RuntimeError, match="max_query_len"):
+        update_block_bounds(bounds, keys, table, starts, torch.tensor([20, 16]).cuda(), 16, max_query_len=19)
+
+
 def select_both(gen, lens, heads, kv_heads, dim, block_size, take, *, sink=1, recent=1, dtype=torch.bfloat16,
                 levels=None, spoil=None, query=None, validate=True, pool_lens=None):
     table, blocks = tables_for(gen, pool_lens or lens, block_size)

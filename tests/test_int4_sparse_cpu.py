@@ -254,3 +254,13 @@ def test_decode_step_checks_its_pool():
             Qwen3DecodeStep(cfg, weights, pool, selected_blocks=4)
     with pytest.raises(ValueError, match="2 blocks"):
         Qwen3DecodeStep(cfg, weights, INT4KVCachePool(*shape, device="cpu", block_bounds=True), selected_blocks=1)
+
+
+def test_decode_refuses_lists_of_more_tiles_than_it_counts():
+    lib = _lib.load()
+    for args in ((40000, 1, 1, 32, 1, 1048576, 1), (1, 65535, 65535, 32, 1, 1, 1048576),
+                 (16384, 1024, 1, 32, 1, 1048576, 1)):
+        for sizer in (lib.minikv_paged_decode_int4_workspace_bytes, lib.minikv_paged_decode_selected_workspace_bytes):
+            assert sizer(*args, _lib.BF16) == -1
+            assert "too large" in lib.minikv_last_error().decode()
+    assert lib.minikv_paged_decode_int4_workspace_bytes(1024, 64, 8, 128, 1 << 20, 16, 65536, _lib.BF16) > 0
