@@ -697,9 +697,10 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 
     const int64_t t0 = team * total / G;
     const int run = (int)((team + 1) * total / G - t0);  // the team's tiles; its warp r takes tiles r, r + TW, ...
 
+    const int searched = (B - 1) / per;  // the last thread that has requests
     auto cursor_at = [&](int64_t t) -> TileCursor {
         const int64_t x = t / U;  // tiles of the requests before (and of the own one's units, divided)
-        int lo = 0, hi = W * 32 - 1;
+        int lo = 0, hi = searched;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (prefix[mid] <= x) lo = mid; else hi = mid - 1;
@@ -896,7 +897,8 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 
     look_page();
     if constexpr (ALIGNED) keep_batch();
 #pragma unroll 1
-    for (int s = 0; s < NS - 1; ++s) copy_tile();
+    for (int s = 0; s < NS; ++s) copy_tile();
+    bool first = true;  // the warp's first tile frees no stage
 
     Consumer c;
     c.setup(lane);
@@ -912,9 +914,10 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 
         const int64_t qh0 = (int64_t)seg.b * p.q_heads + kvh * p.group + 8 * chunk;
         c.begin(static_cast<const T*>(p.q) + qh0 * D, heads, p.scale_log2);
         for (; t < end; t += TW) {
-            copy_wait<NS - 2>();
+            if (first) copy_wait<NS - 1>(); else copy_wait<NS - 2>();
             __syncwarp();  // the stage is whole, and the one filled next has been read by every lane
-            copy_tile();
+            if (!first) copy_tile();
+            first = false;
             c.tile(ring + stage, *reinterpret_cast<const uint32_t*>(ring + stage + Consumer::kStageBytes), p.scale_log2,
                    scratch);
             stage = stage == (NS - 1) * STAGE ? 0 : stage + STAGE;
