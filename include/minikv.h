@@ -378,7 +378,8 @@ int minikv_paged_prefill_int4(const void* q, const void* key_cache, const void* 
  * context_lens[r].  key_cache: [num_blocks, block_size, kv_heads, head_dim] of
  * the dtype `pool`, or a 4-bit pool (pool = MINIKV_INT4).  max_query_len bounds
  * context_lens[r] - query_starts[r]; blocks past the bound are not updated.
- * Requests and pages out of range are skipped. */
+ * Requests and pages out of range are skipped.  A page that several requests
+ * name has to hold the same rows for each of them. */
 int minikv_block_bounds_update(void* bounds, const void* key_cache, const int64_t* block_tables,
                                const int64_t* query_starts, const int64_t* context_lens, int64_t requests,
                                int64_t table_width, int64_t num_blocks, int64_t block_size, int64_t kv_heads,

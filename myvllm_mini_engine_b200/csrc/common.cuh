@@ -26,9 +26,9 @@
 namespace minikv {
 
 // Device status word, read and cleared by minikv_device_status().
-// Bit values are listed in include/minikv.h (MINIKV_STATUS_*).  The library
-// is one translation unit (abi.cu includes the kernel files), so the word is
-// defined here once.
+// Bit values are listed in include/minikv.h (MINIKV_STATUS_*).  The kernels
+// with bounded waits are all in abi.cu's translation unit, whose word this is
+// (pages_abi.cu's kernels wait for nothing but their own asynchronous copies).
 __device__ unsigned int g_status = 0;
 
 __device__ __forceinline__ void raise_status(unsigned int bit) { atomicOr(&g_status, bit); }

@@ -24,15 +24,16 @@
 // a fixed order.  A unit that spans CTAs leaves one partial per CTA; the CTA
 // that takes the unit's last ticket joins them, in the order of the CTAs.
 //
-// Long batches are bound by the instructions that make the operands: about 580
-// a tile of 32 tokens at D = 128, of the 760 that the SM issues in the time that
-// its share of the memory's rate brings the tile (256 requests of 4096 tokens, 8
-// kv heads: 235 us, 4.9 TB/s of the pool, against 177 us at the measured copy
-// rate); small ones by the chain of launch, look-ups, pages and join (8 x 513:
-// 12 us).  Copies a lane rather than bulk copies of a page's head (1 KB at D =
-// 128, block_size 16): both reach the memory's rate here, and these need no
-// barrier and no producer.  mma.sync rather than tcgen05: the group's few query
-// heads are the N = 8 columns, and the operands are made in registers.
+// Long batches are bound by the instructions that make the operands: 631 a
+// tile of 32 tokens at D = 128, where the SM could issue 760 in the time that its
+// share of the memory's rate brings the tile, and the 16 warps that the registers
+// allow keep it at half of that (256 requests of 4096 tokens, 8 kv heads: 230 us,
+// 5.0 TB/s of the pool, against 177 us at the measured copy rate).  Small ones are
+// bound by the chain of launch, look-ups, pages and join (8 x 513: 11.6 us).
+// Copies a lane rather than bulk copies of a slice (1 KB of codes at D = 128):
+// those took 254 us, with more instructions, for the barriers.  mma.sync rather
+// than tcgen05: the group's few query heads are the N = 8 columns, and the
+// operands are made in registers.
 #pragma once
 
 #include "common.cuh"
@@ -568,7 +569,8 @@ struct __align__(16) PageSlice {
     uint32_t mask;
 };
 
-constexpr int kMostPartials = 3;  // of a unit that warps work on alone (measured: see page_decode_kernel)
+// Warps of a 4-bit pool's decode work alone where each gets this many tiles, and no unit more partials than this.
+constexpr int kLeastAlone = 5, kMostPartials = 8;
 
 // Joins n partials of a unit, in their order, into its output rows: `threads` threads share the
 // heads x D elements, four each at a time.  Up to four partials are loaded at once.
@@ -679,18 +681,23 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 
     }
     // ---- teams and their runs of tiles.  A team is the CTA, whose warps take the tiles of its run in
     // turn and join at the end of each unit, or a single warp with a run of its own: no barrier, an
-    // eighth of the joins, but a unit is then cut into as many partials as warps share it.  Warps
-    // where that is at most kMostPartials; both figures come from the lengths, so all CTAs agree.
+    // eighth of the joins, but a unit is then cut into as many partials as warps share it.  The figures
+    // come from the lengths, so all CTAs agree.  A CTA and a warp, D = 128, 8 kv heads: 256 x 4096 tokens
+    // (111 tiles a warp, 2 partials) 266 and 230 us, 64 x 4096 (28, 5) 82 and 75, 64 lists of 1024 (7, 5)
+    // 37 and 33, 32 x 4096 (14, 10) 49 and 47, 32 lists of 2048 (7, 10) 33 and 35, 12 x 4096 (5, 25) 29 and
+    // 31, 32 x 1024 (3.5, 10) 19 and 23, 1 x 131072 (14, 296) 47 and 108.  A 16-bit pool's four warps are
+    // faster together: 64 lists of 2048 tokens 99 and 101 us, 32 of them 57 and 61.
     const int64_t total = (int64_t)prefix[W * 32] * U;
     int longest = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) longest = max(longest, warp_most[w]);
-    const bool alone = (int64_t)longest * gridDim.x * W <= kMostPartials * total;
+    const int64_t slots = (int64_t)gridDim.x * W;
+    const bool alone = INT4 && total >= kLeastAlone * slots && longest * slots <= kMostPartials * total;
     const int TW = alone ? 1 : W, rank = alone ? 0 : warp;  // warps of the team, and this one's place
     const int64_t team = alone ? (int64_t)blockIdx.x * W + warp : blockIdx.x;
     int64_t G = (int64_t)gridDim.x * (alone ? W : 1);  // runs
     // Every run has a tile, of a CTA at least one for each warp; where that is no more than four a warp,
-    // a whole unit's, which then needs no join (8 x 513 tokens: 17.8 -> 12.3 us).
+    // a whole unit's, which then needs no join (8 x 513 tokens: 17.8 -> 11.6 us).
     const int least = longest <= 4 * W ? max(W, longest) : W;
     G = min(G, alone ? total : (total + least - 1) / least);
     if (team >= G) return;

@@ -397,6 +397,8 @@ class Qwen3DecodeStep:
         shape = (batch, 1, cfg.num_key_value_heads, cfg.head_dim)
         self._stage_k = torch.empty(shape, dtype=self.weights.embed.dtype, device=device)
         self._stage_v = torch.empty_like(self._stage_k)
+        if self.int4 or self.selected_blocks is not None:
+            self._lengths = positions + 1
         key = (batch, device)
         if key not in self._stage_index:  # read-only index tensors: made once per batch size
             self._stage_index[key] = (torch.arange(batch, dtype=torch.long, device=device).view(batch, 1),
@@ -429,7 +431,7 @@ class Qwen3DecodeStep:
 
     def _attend_pages(self, index, q, block_tables, positions, stage_k, stage_v):
         """Append, then attend a 4-bit pool, or the blocks selected from the pool's bounds."""
-        pool, lengths = self.pool, positions + 1
+        pool, lengths = self.pool, self._lengths
         if self.int4:
             pool.write_batch(index, block_tables, positions, stage_k, stage_v, validate=False)
         else:

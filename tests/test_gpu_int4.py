@@ -178,6 +178,40 @@ def test_decode_of_more_requests_than_threads(cuda_device):
     assert not actual[lens <= 0].any()
 
 
+@pytest.mark.parametrize("dtype,dim,block_size,select", [
+    (torch.bfloat16, 32, 16, False), (torch.float16, 64, 16, True), (torch.float16, 32, 5, False),
+    (torch.bfloat16, 128, 16, False), (torch.bfloat16, 256, 16, False)])
+def test_decode_of_long_batches(cuda_device, dtype, dim, block_size, select):
+    """Enough tiles that warps work on runs of their own, with partials of a unit in several CTAs."""
+    gen = np.random.default_rng(dim + block_size)
+    batch, heads, kv_heads, longest = 260, 8, 8, 600
+    lens = torch.from_numpy(np.linspace(longest, 300, batch).round().astype(np.int64)[gen.permutation(batch)])
+    lens[100:103] = 0
+    lens[200] = 1
+    width = -(-longest // block_size)
+    kp, vp = make_pool(gen, 30, block_size, kv_heads, dim), make_pool(gen, 30, block_size, kv_heads, dim)
+    table = torch.from_numpy(gen.integers(0, 30, size=(batch, width)).astype(np.int64))
+    selected = None
+    if select:  # all blocks but every third
+        listed = torch.tensor([j for j in range(width) if j % 3])
+        listed = listed.expand(batch, kv_heads, -1).clone()
+        listed[listed * block_size >= lens[:, None, None]] = -1
+        selected = listed.contiguous()
+    tiles = lens if selected is None else (selected >= 0).sum(-1)[:, 0] * block_size
+    warps = torch.cuda.get_device_properties(0).multi_processor_count * 16
+    assert int((tiles // 32).sum()) * kv_heads >= 5 * warps
+    query = randn(gen, batch, heads, dim).to(dtype)
+    keys, vals = int4_kv.values(kp, block_size, dim), int4_kv.values(vp, block_size, dim)
+    expected = int4_kv.paged_decode(query, keys, vals, table, lens, block_size, selected)
+    args = [x.cuda() for x in (query, torch.from_numpy(kp), torch.from_numpy(vp), table, lens)]
+    listed = None if selected is None else selected.cuda()
+    actual = paged_attention_int4(*args, block_size, selected=listed, validate=False)
+    assert_near(actual, expected, query, keys, vals, dtype, dtype == torch.bfloat16)
+    assert not actual[100:103].any()
+    for _ in range(3):  # partials are joined in one order
+        assert torch.equal(paged_attention_int4(*args, block_size, selected=listed, validate=False), actual)
+
+
 @pytest.mark.parametrize("scale,q_scale", [(2.0 ** -12, 1.0), (3000.0, 2.0 ** -8), (1.0, 2.0 ** -40), (2.0 ** -9, 2.0 ** 30)])
 def test_decode_extreme_scales(cuda_device, scale, q_scale):
     decode(np.random.default_rng(9), torch.bfloat16, (40, 700), 8, 2, 64, 16, scale=scale, q_scale=q_scale)
