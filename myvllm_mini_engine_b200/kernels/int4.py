@@ -16,8 +16,8 @@ row (one token, one kv head, K or V by itself), and read as ``base + step * code
 NaN counts as 0 and magnitudes saturate at 65504.  At head_dim 128 that is 4.25
 bits an element: a decode step streams 68 bytes where a 16-bit pool has 256.
 
-The decode's scratch memory is kept per stream for eager calls; a captured graph
-gets its own.
+The decode's scratch memory is kept per stream for eager calls; a captured call
+has its own.
 """
 
 from __future__ import annotations
@@ -231,6 +231,22 @@ def read_kv_cache_slots_int4(key_cache, value_cache, slot_mapping, block_size, h
 _NEEDS: dict = {}
 _SCRATCH: dict = {}
 _OLD_SCRATCH: list = []
+_CAPTURED: dict = {}
+_CAPTURED_TICKETS = 1 << 22
+
+
+def _captured_tickets(device, count):
+    """Counters of one captured call: zero, as every launch of it leaves them, and never another call's.
+
+    They come from a buffer that the first eager call on the device zeroed, so that
+    a replay need not; once that is used up (or before an eager call) the graph
+    holds counters that it zeroes itself, about 2 us a call.
+    """
+    held = _CAPTURED.get(device.index)
+    if held is None or held[1] + count > held[0].numel():
+        return torch.zeros(count, dtype=torch.int32, device=device)
+    first, held[1] = held[1], held[1] + count
+    return held[0][first:first + count]
 
 
 def _scratch(device, stream, tickets, need):
@@ -238,15 +254,18 @@ def _scratch(device, stream, tickets, need):
 
     Every launch leaves the counters zero, whatever its shape, and the workspace
     may hold anything, so the eager calls on one stream, which follow one another,
-    share them.  A captured graph may run beside other work of its stream: it gets
-    its own, from the graph's memory, zeroed inside the graph.
+    share them.  A captured call may run beside other work of its stream: it gets
+    counters of its own, and a workspace from the graph's memory.
     """
     if torch.cuda.is_current_stream_capturing():
-        return (torch.zeros(tickets, dtype=torch.int32, device=device),
-                torch.empty(need, dtype=torch.uint8, device=device))
+        return _captured_tickets(device, tickets), torch.empty(need, dtype=torch.uint8, device=device)
     key = (device.index, stream)
     held = _SCRATCH.get(key)
     if held is None or held[0].numel() < tickets or held[1].numel() < need:
+        if device.index not in _CAPTURED:
+            zeros = torch.zeros(_CAPTURED_TICKETS, dtype=torch.int32, device=device)
+            torch.cuda.current_stream(device).synchronize()  # once: a replay may run on any stream
+            _CAPTURED[device.index] = [zeros, 0]
         if held is not None:
             _OLD_SCRATCH.append(held)  # a launch in flight may still use it
             tickets, need = max(tickets, 2 * held[0].numel()), max(need, 2 * held[1].numel())

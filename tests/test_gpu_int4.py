@@ -358,6 +358,35 @@ def test_decode_on_other_streams_and_in_graphs(cuda_device):
 
 # ------------------------------------------------------------------ prefill
 
+@pytest.mark.parametrize("left", [0, 20, 1 << 20])
+def test_captured_calls_have_counters_of_their_own(cuda_device, monkeypatch, left):
+    """Graphs of several decodes that run at the same time, with kept counters or with the graph's own."""
+    from myvllm_mini_engine_b200.kernels import int4
+
+    gen = np.random.default_rng(31)
+    table, blocks = tables_for(gen, [3000, 900], 16)
+    kp, vp = (torch.from_numpy(make_pool(gen, blocks, 16, 2, 64)).cuda() for _ in range(2))
+    lens, table = torch.tensor([3000, 900]).cuda(), table.cuda()
+    query = [randn(gen, 2, 4, 64).to(torch.float16).cuda() for _ in range(6)]
+    run = lambda q: paged_attention_int4(q, kp, vp, table, lens, 16, validate=False)  # noqa: E731
+    expected = [run(q) for q in query]
+    counters, used = int4._CAPTURED[torch.cuda.current_device()]
+    monkeypatch.setitem(int4._CAPTURED, torch.cuda.current_device(), [counters, max(used, counters.numel() - left)])
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for part in (query[:3], query[3:]):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs += [run(q) for q in part]
+    for _ in range(20):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for out, want in zip(outs, expected):
+        assert torch.equal(out, want)
+    assert not counters.any()
+
+
 def prefill(gen, dtype, counts, starts, heads, kv_heads, dim, block_size, *, tables=None, lens=None, extra=0,
             validate=True, scale=1.0, max_query_len=None):
     full = [s + c for s, c in zip(starts, counts)]
