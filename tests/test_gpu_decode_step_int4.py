@@ -1,6 +1,6 @@
 """The Qwen3 decode step over a 4-bit pool and over selected blocks, and the pools' own methods.
 
-Checker: the same step with its attention in plain PyTorch over the rows that it
+Compared with the same step with its attention in plain PyTorch over the rows that it
 reads back from its own copy of the pool (the writes, the bounds and the
 selection have tests of their own against the 64-bit oracle).  Both steps round
 the attention's result to bf16, so from the second layer on they differ by that
