@@ -346,12 +346,10 @@ int minikv_paged_decode_int4(const void* query, const void* key_cache, const voi
 
 /* Ragged causal prefill over a 4-bit pool: minikv_paged_prefill's contract with
  * an fp16/bf16 query and output and up to 64 query heads a kv head.  Tokens of
- * no request, or past their context, get zero rows.  Two routes: the codes as
- * operands, exact, for every shape; and, for bf16 batches of enough queries a
- * request on the tcgen05 prefill's shapes, that kernel on an fp16 copy of the
- * pages the tables reference (base + step * code rounded to fp16, Q saturated to
- * fp16's range), made in the workspace (256-byte aligned; 0 bytes on the other
- * route, where none is read). */
+ * no request, or past their context, get zero rows.  The codes are operands as
+ * they are, and a request's rows do not depend on the rest of the batch or on
+ * the table's width.  No workspace is read: its size is 0, or -1 for a shape
+ * that the call refuses. */
 int64_t minikv_paged_prefill_int4_workspace_bytes(int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
                                                   int64_t head_dim, int64_t num_blocks, int64_t block_size,
                                                   int64_t table_width, int dtype);

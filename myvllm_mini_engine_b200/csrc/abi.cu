@@ -762,6 +762,3 @@ int minikv_linear_qk_rope_append(const void* x, int64_t x_stride, const float* s
 // The no-allocation decode entry point (its scratch array and its set-up live in
 // that file; it uses check_decode_shapes above).
 #include "decode_noalloc.cu"
-
-// The 4-bit prefill's route over the tcgen05 kernel (its entry point is in pages_abi.cu).
-#include "prefill_int4_dense.cu"

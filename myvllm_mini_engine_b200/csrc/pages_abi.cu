@@ -15,13 +15,6 @@
 
 // in abi.cu's unit
 extern "C" int minikv_set_error(int code, const char* message);
-extern "C" int64_t minikv_prefill_int4_dense_bytes(int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
-                                                   int64_t head_dim, int64_t block_size, int64_t width, int dtype);
-extern "C" int minikv_prefill_int4_dense(const void* q, const void* key_cache, const void* value_cache,
-                                         const int64_t* cu, const int64_t* starts, const int64_t* tables,
-                                         const int64_t* lens, void* out, void* workspace, int64_t tokens,
-                                         int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-                                         int64_t num_blocks, int64_t block_size, int64_t width, int dtype, void* stream);
 
 namespace {
 
@@ -351,14 +344,12 @@ int64_t minikv_paged_prefill_int4_workspace_bytes(int64_t tokens, int64_t reques
                                                   int64_t table_width, int dtype) {
     if (check_prefill(tokens, requests, q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, dtype))
         return -1;
-    if (tokens == 0) return 0;
-    return std::max<int64_t>(0, minikv_prefill_int4_dense_bytes(tokens, requests, q_heads, kv_heads, head_dim, block_size,
-                                                                table_width, dtype));
+    return 0;
 }
 
 int minikv_paged_prefill_int4(const void* q, const void* key_cache, const void* value_cache,
                               const int64_t* cu_seqlens_q, const int64_t* query_starts, const int64_t* block_tables,
-                              const int64_t* context_lens, void* out, void* workspace, int64_t workspace_bytes,
+                              const int64_t* context_lens, void* out, void* /*workspace*/, int64_t /*workspace_bytes*/,
                               int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                               int64_t num_blocks, int64_t block_size, int64_t table_width, int64_t max_query_len,
                               int dtype, void* stream) {
@@ -372,15 +363,6 @@ int minikv_paged_prefill_int4(const void* q, const void* key_cache, const void* 
                   MINIKV_EINVAL, "null pointer argument");
     PAGES_REQUIRE(aligned16(q) && aligned16(key_cache) && aligned16(value_cache) && aligned16(out), MINIKV_EINVAL,
                   "paged prefill tensors must be 16-byte aligned");
-    const int64_t dense = minikv_prefill_int4_dense_bytes(tokens, requests, q_heads, kv_heads, head_dim, block_size,
-                                                          table_width, dtype);
-    if (dense >= 0) {
-        PAGES_REQUIRE(workspace && workspace_bytes >= dense && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
-                      MINIKV_EINVAL, "paged prefill workspace too small or misaligned");
-        return minikv_prefill_int4_dense(q, key_cache, value_cache, cu_seqlens_q, query_starts, block_tables,
-                                         context_lens, out, workspace, tokens, requests, q_heads, kv_heads, head_dim,
-                                         num_blocks, block_size, table_width, dtype, stream);
-    }
     const int64_t group = q_heads / kv_heads;
     PrefillInt4Params p{};
     p.q = q;

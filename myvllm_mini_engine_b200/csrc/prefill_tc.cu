@@ -220,13 +220,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_tc_kernel(
     using L = PfLayout<T, D>;
     constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
     // F8 = 1 (E4M3) or 2 (E5M2): K/V come from an FP8 pool through pf_convert_codes, and
-    // the MMAs run in fp16 (a bf16 query tile is converted once per item).  F8 = 3: Q, K and V
-    // are fp16 whatever the output's type T
-    constexpr bool kCodes = F8 == 1 || F8 == 2;
-    static_assert(!kCodes || D == 128, "FP8 pages are staged for head_dim 128 only");
+    // the MMAs run in fp16 (a bf16 query tile is converted once per item)
+    static_assert(F8 == 0 || D == 128, "FP8 pages are staged for head_dim 128 only");
     using C = typename std::conditional<F8 != 0, __half, T>::type;  // MMA operand type
     constexpr bool kMmaBf16 = F8 == 0 && kBf16;
-    constexpr bool kConvertQ = kCodes && kBf16;
+    constexpr bool kConvertQ = F8 != 0 && kBf16;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char* sQ = smem;
@@ -351,7 +349,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) paged_prefill_tc_kernel(
     const int c = blockIdx.x, nC = gridDim.x;
 
     if (warp == 0 || warp == kPfVWarp) {
-        if constexpr (kCodes) {
+        if constexpr (F8 != 0) {
             // -------------------------------------------------------- FP8 producers
             // As below, with a tile's codes (one box of R rows x 128 bytes per page)
             // landing on k8_full / v8_full; the warp converts tile g after issuing the
@@ -886,21 +884,18 @@ static int run_prefill_tc(const void* q, const void* key_cache, const void* valu
                           void* out, int64_t tokens, int64_t requests, int64_t q_heads, int64_t kv_heads,
                           int64_t head_dim, int64_t num_blocks, int64_t block_size, int64_t table_width, int dtype,
                           cudaStream_t stream, double k_scale = 1.0, float v_scale = 1.f, int f8 = 0) {
-    // f8: 0 = 16-bit pool; 1 / 2 = E4M3 / E5M2 pool (head_dim 128), codes converted in the kernel;
-    // 3 = Q, K and V in fp16, a bf16 output
-    const bool codes = f8 == 1 || f8 == 2;
-    if (codes && head_dim != 128) return fail(MINIKV_EINVAL, "FP8 pages are staged for head_dim 128 only");
+    // f8: 0 = 16-bit pool; 1 / 2 = E4M3 / E5M2 pool (head_dim 128), codes converted in the kernel
+    if (f8 != 0 && head_dim != 128) return fail(MINIKV_EINVAL, "FP8 pages are staged for head_dim 128 only");
     const bool bf16 = dtype == MINIKV_BF16;
     const int group = (int)(q_heads / kv_heads);
     const int tm = 128 / group;
     const int box_rows = gcd_int((int)std::min<int64_t>(block_size, 1 << 20), 128);
     CUtensorMap mq, mk, mv;
-    const bool map16 = bf16 && f8 != 3;
-    if (!encode_map_3d(&mq, q, map16, head_dim, q_heads, tokens, 64, group, tm) ||
-        (!codes &&
-         (!encode_map_3d(&mk, key_cache, map16, head_dim, kv_heads, num_blocks * block_size, 64, 1, box_rows) ||
-          !encode_map_3d(&mv, value_cache, map16, head_dim, kv_heads, num_blocks * block_size, 64, 1, box_rows))) ||
-        (codes &&
+    if (!encode_map_3d(&mq, q, bf16, head_dim, q_heads, tokens, 64, group, tm) ||
+        (f8 == 0 &&
+         (!encode_map_3d(&mk, key_cache, bf16, head_dim, kv_heads, num_blocks * block_size, 64, 1, box_rows) ||
+          !encode_map_3d(&mv, value_cache, bf16, head_dim, kv_heads, num_blocks * block_size, 64, 1, box_rows))) ||
+        (f8 != 0 &&
          (!encode_map_3d_u8(&mk, key_cache, head_dim, kv_heads, num_blocks * block_size, 128, 1, box_rows) ||
           !encode_map_3d_u8(&mv, value_cache, head_dim, kv_heads, num_blocks * block_size, 128, 1, box_rows))))
         return fail(MINIKV_ECUDA, "cuTensorMapEncodeTiled failed for the paged prefill operands");
@@ -928,10 +923,7 @@ static int run_prefill_tc(const void* q, const void* key_cache, const void* valu
     if ((tokens + tm - 1) / tm + requests >= (1 << 20)) return fail(MINIKV_EINVAL, "too many paged prefill tiles");
     const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(items_bound, sm_count()));
     cudaError_t err;
-    if (f8 == 3) {
-        err = head_dim == 64 ? launch_prefill_tc_typed<__nv_bfloat16, 64, 3>(mq, mk, mv, p, grid, stream)
-                             : launch_prefill_tc_typed<__nv_bfloat16, 128, 3>(mq, mk, mv, p, grid, stream);
-    } else if (f8 != 0) {
+    if (f8 != 0) {
         if (bf16)
             err = f8 == 1 ? launch_prefill_tc_typed<__nv_bfloat16, 128, 1>(mq, mk, mv, p, grid, stream)
                           : launch_prefill_tc_typed<__nv_bfloat16, 128, 2>(mq, mk, mv, p, grid, stream);

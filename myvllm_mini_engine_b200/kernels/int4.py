@@ -378,10 +378,9 @@ def paged_prefill_attention_int4(q, key_cache, value_cache, cu_seqlens_q, query_
     ``q`` is fp16 or bf16 ``[tokens, q_heads, head_dim]`` with up to 64 query heads
     a kv head.  Metadata, checks and messages as ``paged_prefill_attention``
     (``mini_engine/kernels/prefill.py:61-131``).  Packed tokens of no request, or
-    past their context, get zeros.  The codes enter the products exactly, except
-    for bf16 batches with enough queries a request, which run on the tcgen05
-    prefill over an fp16 copy of their pages (rounded to 2^-12, under the output's
-    own 2^-9; Q saturated to fp16's range).
+    past their context, get zeros.  The codes enter the products exactly.  A
+    request's rows do not depend on the batch around it or on the table's width,
+    and the call takes no workspace.
     """
     if backend != "cuda":
         raise ValueError("paged prefill backend must be cuda (this package has no torch/CPU path)")
@@ -425,17 +424,11 @@ def paged_prefill_attention_int4(q, key_cache, value_cache, cu_seqlens_q, query_
     lib = _lib.load()
     _, heads, dim = q.shape
     code, device = _lib.DTYPE_CODES[q.dtype], q.device
-    need = lib.minikv_paged_prefill_int4_workspace_bytes(tokens, requests, heads, kv_heads, dim, num_blocks, block_size,
-                                                         width, code)
-    if need < 0:
-        _lib.check(_lib.EINVAL, "paged_prefill_attention_int4")
     with _lib.on_device(device):
-        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None  # 0: not read
         status = lib.minikv_paged_prefill_int4(
             q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), cu_seqlens_q.data_ptr(),
-            query_starts.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), output.data_ptr(),
-            workspace.data_ptr() if need else None, need, tokens, requests, heads, kv_heads, dim, num_blocks,
-            block_size, width, bound, code, _lib.stream_of(device))
+            query_starts.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), output.data_ptr(), None, 0,
+            tokens, requests, heads, kv_heads, dim, num_blocks, block_size, width, bound, code, _lib.stream_of(device))
     if status:
         _lib.check(status, "paged_prefill_attention_int4")
     return output

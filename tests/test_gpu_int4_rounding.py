@@ -1,0 +1,68 @@
+"""Bits that the 4-bit pool's attention and the selected decode have to keep, against the 64-bit oracle.
+
+An output is the 64-bit value rounded once, off by half a step of its type at that value, plus 2 ``inner`` (twice, for
+values at the border of two binades), where ``inner`` is what is lost before the rounding:
+  weights: lg2.approx is off by 2^-22 relative, so of a step in [2^-6, 2^2] by at most 6 * 2^-22 (log2), which is
+    4.2 * 2^-22 of a weight; ex2.approx by 2^-22, rcp.approx by 2^-23, the two fp16 terms of P' by 2^-22 (hi is
+    nearest, the rest has 11 bits of its own): under 7 * 2^-22; scores of |s| < 3 (log2) that are one product (keys of
+    one value each, a query of one power of two) have three roundings, 9 * 2^-24 ln 2: under 9 * 2^-22 of a weight in
+    all, and twice that of a quotient of two sums;
+  sums: fp32, of a few hundred tokens in at most 16 dependent additions of 2^-23 a warp, and the odd codes' sums are
+    1/16 of a difference of sums 17 times as large, 2^-23 each: under 20 * 2^-23;
+  together under 28 * 2^-22 of the spread of the values, taken as 2^-17;
+  other scores, off by ds (log2): 2 ln 2 ds of the spread, ds = (D + 8) 2^-23 of the sum of the products' magnitudes.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from myvllm_mini_engine_b200.kernels import (int4_page_bytes, paged_attention_int4, paged_attention_selected,
+                                             paged_prefill_attention_int4)
+from oracle import int4_kv
+
+pytestmark = pytest.mark.gpu
+
+
+def randn(gen, *shape):
+    return torch.from_numpy(gen.standard_normal(shape, dtype=np.float32))
+
+
+def pool_of(rows, block_size):
+    """A uint8 pool that holds ``rows [tokens, heads, dim]`` in the order of its slots."""
+    tokens, heads, dim = rows.shape
+    pool = np.zeros((-(-tokens // block_size), heads, int4_page_bytes(block_size, dim)), dtype=np.uint8)
+    int4_kv.scatter(pool, block_size, torch.arange(tokens), rows)
+    return pool
+
+
+def rows_of_many_steps(gen, tokens, heads, dim):
+    """Normal rows, each times a factor of its own."""
+    return (randn(gen, tokens, heads, dim) + randn(gen, heads, dim)) * (0.5 + 1.5 * torch.from_numpy(
+        gen.random((tokens, heads, 1), dtype=np.float32)))
+
+
+def test_prefill_does_not_depend_on_its_neighbours(cuda_device):
+    """bf16: a request alone, in batches of short and of long chunks, and on a wider table gives the same bytes."""
+    gen = np.random.default_rng(8)
+    bs, dim, heads, kv_heads, count, start = 16, 128, 4, 2, 40, 70
+    blocks = 60
+    pools = [torch.from_numpy(pool_of(rows_of_many_steps(gen, blocks * bs, kv_heads, dim), bs)).cuda() for _ in range(2)]
+    table = torch.from_numpy(gen.permutation(blocks).astype(np.int64))
+    q = randn(gen, 400, heads, dim).to(torch.bfloat16).cuda()
+
+    def run(counts, starts, width):
+        cu = torch.tensor([0, *np.cumsum(counts)])
+        tables = torch.full((len(counts), width), -1)
+        for r, (c, s) in enumerate(zip(counts, starts)):
+            used = -(-(c + s) // bs)
+            tables[r, :used] = table[20 * r:20 * r + used]
+        lens = torch.tensor([c + s for c, s in zip(counts, starts)])
+        return paged_prefill_attention_int4(q[:int(cu[-1])].contiguous(), *pools, cu.cuda(), torch.tensor(starts).cuda(),
+                                            tables.cuda(), lens.cuda(), bs)[:count]
+
+    alone = run([count], [start], 7)
+    for counts, starts, width in (([count, 1, 1], [start, 5, 90], 7), ([count, 200], [start, 11], 14), ([count], [start], 60000)):
+        assert torch.equal(run(counts, starts, width), alone)
