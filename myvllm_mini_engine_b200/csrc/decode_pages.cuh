@@ -160,7 +160,13 @@ constexpr float kCodeScale = 16777216.f;       // 2^24: a nibble in the low bits
 // A lane first turns the (step, base) pairs of one token into what the scores
 // and the sums need, for the whole warp: done by every lane for its own rows it
 // took a sixth of the tile's instructions.
-template <typename T, int D>
+// P' goes in as two fp16 terms (2^-22): one (2^-12) would move a twentieth of a
+// bf16 output's roundings to the next value.  TWIN: a unit of up to four heads
+// holds them twice, in columns 0..3 and again in 4..7, so the same scores and P' come
+// out there; those columns multiply the second term, and their sums are added at
+// the unit's end: no MMA more than one term takes (256 x 4096 tokens, D = 128,
+// two heads a kv head, eager: one term 269 us, this 278, a second set of MMAs 293).
+template <typename T, int D, bool TWIN>
 struct Int4Consumer {
     static constexpr int TT = 32;
     static constexpr int RB = D / 2;                         // bytes of a row's codes
@@ -171,9 +177,6 @@ struct Int4Consumer {
     static constexpr int NW = D / 32;                        // words of K a lane takes of a row
     static constexpr int NH = D / 32;                        // 16-bit runs of V a lane takes of a row
     static constexpr int kPieces = NH;                       // groups of 32 output dims
-    // An fp16 output resolves 2^-11: P' then goes in as two fp16 terms (2^-22).  Next to a bf16
-    // output's own rounding of 2^-9 one term (2^-12) is lost, and half of V's MMAs are saved.
-    static constexpr bool kTwoTerms = std::is_same<T, __half>::value;
 
     uint32_t qb[2 * NW][2];
     float o[2 * NH][4];
@@ -191,10 +194,11 @@ struct Int4Consumer {
     __device__ void begin(const T* q, int heads, float scale_log2) {
         float f[8 * NW];
         float top = 0.f;
-        if (g < heads) {
+        const int head = TWIN ? g & 3 : g;
+        if (head < heads) {
 #pragma unroll
             for (int i = 0; i < 8 * NW; i += 8) {
-                Elem<T>::load(*reinterpret_cast<const uint4*>(q + g * D + q4 * (D / 4) + i), f + i);
+                Elem<T>::load(*reinterpret_cast<const uint4*>(q + head * D + q4 * (D / 4) + i), f + i);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[i + e]));
             }
@@ -369,31 +373,40 @@ struct Int4Consumer {
                 z[e & 1] = fmaf(p[e], rbase[i][e >> 1], z[e & 1]);
             }
             const uint32_t p01 = Elem<__half>::pack(p[0], p[1]), p23 = Elem<__half>::pack(p[2], p[3]);
-            const uint32_t b0 = transpose8x8(p01), b1 = transpose8x8(p23);
-            uint32_t c0 = 0, c1 = 0;
-            if constexpr (kTwoTerms) {
-                float back[4];
-                Elem<__half>::unpack(p01, back);
-                Elem<__half>::unpack(p23, back + 2);
-                c0 = transpose8x8(Elem<__half>::pack(p[0] - back[0], p[1] - back[1]));
-                c1 = transpose8x8(Elem<__half>::pack(p[2] - back[2], p[3] - back[3]));
-            }
+            float back[4];
+            Elem<__half>::unpack(p01, back);
+            Elem<__half>::unpack(p23, back + 2);
+            const uint32_t r01 = Elem<__half>::pack(p[0] - back[0], p[1] - back[1]);
+            const uint32_t r23 = Elem<__half>::pack(p[2] - back[2], p[3] - back[3]);
+            const bool second = TWIN && q4 >= 2;
             uint32_t x0[NH], x1[NH];
             const unsigned char* v = vst + (16 * i + q4) * RB + g * (RB / 8);
             load_v(v, v + 4 * RB, x0);
             load_v(v + 8 * RB, v + 12 * RB, x1);
+            add_values(x0, x1, transpose8x8(second ? r01 : p01), transpose8x8(second ? r23 : p23));
+            if constexpr (!TWIN) add_values(x0, x1, transpose8x8(r01), transpose8x8(r23));
+        }
+    }
+
+    // O of 16 tokens
+    __device__ __forceinline__ void add_values(const uint32_t* x0, const uint32_t* x1, uint32_t b0, uint32_t b1) {
 #pragma unroll
-            for (int u = 0; u < NH; ++u) {
-                const uint32_t b[4] = {x0[u] & 0x00ff00ffu, permute_bytes(x0[u], 0u, 0x4341u), x1[u] & 0x00ff00ffu,
-                                       permute_bytes(x1[u], 0u, 0x4341u)};
-                const uint32_t a[4] = {b[0] & kNibbleMask, b[1] & kNibbleMask, b[2] & kNibbleMask, b[3] & kNibbleMask};
-                mma16816<__half>(o[2 * u], a, b0, b1);
-                mma16816<__half>(o[2 * u + 1], b, b0, b1);
-                if constexpr (kTwoTerms) {
-                    mma16816<__half>(o[2 * u], a, c0, c1);
-                    mma16816<__half>(o[2 * u + 1], b, c0, c1);
-                }
-            }
+        for (int u = 0; u < NH; ++u) {
+            const uint32_t b[4] = {x0[u] & 0x00ff00ffu, permute_bytes(x0[u], 0u, 0x4341u), x1[u] & 0x00ff00ffu,
+                                   permute_bytes(x1[u], 0u, 0x4341u)};
+            const uint32_t a[4] = {b[0] & kNibbleMask, b[1] & kNibbleMask, b[2] & kNibbleMask, b[3] & kNibbleMask};
+            mma16816<__half>(o[2 * u], a, b0, b1);
+            mma16816<__half>(o[2 * u + 1], b, b0, b1);
+        }
+    }
+
+    // A unit's end: the second terms' sums join the first ones'.
+    __device__ __forceinline__ void finish() {
+        if constexpr (TWIN) {
+#pragma unroll
+            for (int x = 0; x < 2 * NH; ++x)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[x][i] += __shfl_xor_sync(0xffffffffu, o[x][i], 2);
         }
     }
 
@@ -518,6 +531,8 @@ struct Wide16Consumer {
             mma16816<T>(o[k], a, b0, b1);
         }
     }
+
+    __device__ __forceinline__ void finish() {}
 
     __device__ __forceinline__ void put_piece(int u, const float* f, float* dst) const {
 #pragma unroll
@@ -929,6 +944,7 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 
                    scratch);
             stage = stage == (NS - 1) * STAGE ? 0 : stage + STAGE;
         }
+        c.finish();
         const bool whole = seg.j == 0 && end - done == seg.tiles;
         const int64_t unit = (int64_t)seg.b * U + seg.ul;
         const int64_t record = unit + team;  // grows by at least one from segment to segment

@@ -144,13 +144,14 @@ int check_tiles(int64_t batch, int64_t q_heads, int64_t block_size, int64_t widt
 }
 
 // Calls f with the consumer type and whether the pool is 4-bit.
-template <typename F> auto with_consumer(bool int4, int dtype, int64_t dim, F f) {
+template <typename F> auto with_consumer(bool int4, int dtype, int64_t dim, int64_t group, F f) {
     return with_type16(dtype, [&](auto t) {
         return with_dim(dim, [&](auto d) {
             using T = typename decltype(t)::type;
             constexpr int D = decltype(d)::value;
-            return int4 ? f(TypeTag<Int4Consumer<T, D>>(), t, d, std::true_type())
-                        : f(TypeTag<Wide16Consumer<T, D>>(), t, d, std::false_type());
+            if (!int4) return f(TypeTag<Wide16Consumer<T, D>>(), t, d, std::false_type());
+            return group <= 4 ? f(TypeTag<Int4Consumer<T, D, true>>(), t, d, std::true_type())
+                              : f(TypeTag<Int4Consumer<T, D, false>>(), t, d, std::true_type());
         });
     });
 }
@@ -158,7 +159,7 @@ template <typename F> auto with_consumer(bool int4, int dtype, int64_t dim, F f)
 void decode_plan(bool int4, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int dtype,
                  PageDecodePlan* plan) {
     const int sms = sm_count();
-    with_consumer(int4, dtype, dim, [&](auto c, auto, auto, auto i) {
+    with_consumer(int4, dtype, dim, q_heads / kv_heads, [&](auto c, auto, auto, auto i) {
         page_decode_plan<typename decltype(c)::type, decltype(i)::value>(batch, q_heads, kv_heads, dim, sms, plan);
         return 0;
     });
@@ -221,7 +222,7 @@ int run_page_decode(bool int4, const void* query, const void* key_cache, const v
         p.page_stride = block_size * p.row_stride;
     }
     p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)dim));
-    const cudaError_t err = with_consumer(int4, dtype, dim, [&](auto c, auto t, auto d, auto i) {
+    const cudaError_t err = with_consumer(int4, dtype, dim, q_heads / kv_heads, [&](auto c, auto t, auto d, auto i) {
         using C = typename decltype(c)::type;
         using T = typename decltype(t)::type;
         constexpr int D = decltype(d)::value;

@@ -38,10 +38,46 @@ def pool_of(rows, block_size):
     return pool
 
 
+def half_step(x, dtype):
+    bits, least = (10, -14) if dtype == torch.float16 else (7, -126)
+    exponent = torch.frexp(x.abs()).exponent.double() - 1
+    return torch.exp2(exponent.clamp(min=least) - bits - 1)
+
+
+def assert_rounded_once(actual, expected, inner, dtype):
+    err = (actual.double().cpu() - expected).abs()
+    over = err - half_step(expected, dtype) - 2 * inner
+    assert bool((over <= 0).all()), (int((over > 0).sum()), float(over.max()), float(err.max()))
+
+
 def rows_of_many_steps(gen, tokens, heads, dim):
     """Normal rows, each times a factor of its own."""
     return (randn(gen, tokens, heads, dim) + randn(gen, heads, dim)) * (0.5 + 1.5 * torch.from_numpy(
         gen.random((tokens, heads, 1), dtype=np.float32)))
+
+
+def keys_of_one_value(gen, tokens, heads, dim):
+    """Rows of one fp16 value in (-1, 1) each: with a query of 1/8 everywhere a score is that value times sqrt(dim) / 8."""
+    return torch.from_numpy(gen.uniform(-1, 1, (tokens, heads, 1)).astype(np.float16)).float().expand(-1, -1, dim)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,select,heads,kv_heads", [(32, False, 8, 4), (64, True, 12, 2), (128, False, 8, 4),
+                                                       (128, True, 14, 2), (128, False, 9, 1), (256, False, 4, 1)])
+def test_decode_weights_keep_their_bits(cuda_device, dtype, dim, select, heads, kv_heads):
+    gen = np.random.default_rng(dim)
+    bs, lens = 16, torch.tensor([1, 2, 3, 5, 17, 40, 130])
+    width = 9
+    rows = len(lens) * width * bs, kv_heads, dim
+    kp, vp = pool_of(keys_of_one_value(gen, *rows), bs), pool_of(rows_of_many_steps(gen, *rows), bs)
+    table = torch.from_numpy(gen.permutation(len(lens) * width).astype(np.int64)).view(len(lens), width)
+    keys, vals = int4_kv.values(kp, bs, dim), int4_kv.values(vp, bs, dim)
+    query = torch.full((len(lens), heads, dim), 0.125, dtype=dtype)
+    selected = torch.arange(width).expand(len(lens), kv_heads, width).contiguous() if select else None
+    expected = int4_kv.paged_decode(query, keys, vals, table, lens, bs)
+    actual = paged_attention_int4(query.cuda(), *(torch.from_numpy(p).cuda() for p in (kp, vp)), table.cuda(), lens.cuda(),
+                                  bs, validate=False, selected=None if selected is None else selected.cuda())
+    assert_rounded_once(actual, expected, float(vals.max() - vals.min()) * 2.0 ** -17, dtype)
 
 
 def test_prefill_does_not_depend_on_its_neighbours(cuda_device):
