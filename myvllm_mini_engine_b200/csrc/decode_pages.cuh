@@ -138,6 +138,17 @@ __device__ __forceinline__ float column_sum(float x) {
 // only then: a vote tells.
 constexpr float kMaxSlack = 8.f;
 
+// The fp16 query of a 4-bit pool is scaled by a power of two so that a row's largest element lies in
+// [2^14, 2^15): elements keep all of their bits down to 2^-24 of the largest (odd ones, stored 16 times
+// smaller, too), and below that are off by 2^-35 of it at most.
+constexpr int kQueryTop = 14;
+// The exponent of the largest element less kQueryTop, kept where 2^-e and 2^e are both normal.
+__device__ __forceinline__ int query_exponent(float top) {
+    const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127 - kQueryTop;
+    return top > 0.f && top < INFINITY ? min(120, max(-120, e)) : 0;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
 constexpr uint32_t kNibbleMask = 0x000f000fu;  // the low nibbles of two halves
 constexpr float kCodeScale = 16777216.f;       // 2^24: a nibble in the low bits of a half is code 2^-24
 
@@ -189,8 +200,7 @@ struct Int4Consumer {
         q4 = lane & 3;
     }
 
-    // Q of head g in fp16, scaled by a power of two so that its largest magnitude lies in [1, 2): bf16
-    // values keep their bits then, whatever their exponents.
+    // Q of head g in fp16, scaled (kQueryTop)
     __device__ void begin(const T* q, int heads, float scale_log2) {
         float f[8 * NW];
         float top = 0.f;
@@ -208,16 +218,14 @@ struct Int4Consumer {
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // exponent of the largest element, kept where 2^-e and 2^e are both normal
-        const int e = (top > 0.f && top < INFINITY) ? min(120, max(-120, (int)((__float_as_uint(top) >> 23) & 255) - 127)) : 0;
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        const int e = query_exponent(top);
+        const float down = power_of_two(-e);
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                // fp16 below 2^-14 of the largest element rounds to 2^-24 of it (odd nibbles: 2^-20)
                 const float unit = (i & 1) ? 0.0625f : 1.f;
                 x[i] = __half2float(__float2half_rn(f[8 * w + i] * down * unit));
                 sum += (i & 1) ? x[i] * 16.f : x[i];
@@ -229,7 +237,7 @@ struct Int4Consumer {
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const float up = __uint_as_float((uint32_t)(127 + e) << 23) * scale_log2;
+        const float up = power_of_two(e) * scale_log2;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {  // of the heads this lane's accumulators hold
             qsum[h] = __shfl_sync(0xffffffffu, sum, (2 * q4 + h) * 4);

@@ -110,25 +110,18 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // scaled by a power of two into [1, 2), as in the decode
-            const int e2 = (top > 0.f && top < INFINITY)
-                               ? min(120, max(-120, (int)((__float_as_uint(top) >> 23) & 255) - 127)) : 0;
-            const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+            const int e2 = query_exponent(top);  // scaled as in the decode
+            const float down = power_of_two(-e2);
             float sum = 0.f;
 #pragma unroll
             for (int w = 0; w < NW; ++w) {
                 float y[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    y[i] = __half2float(__float2half_rn(f[8 * w + i] * down));
                     // the operand of a high nibble, 16 times larger as a subnormal
-                    if (i & 1) {
-                        const float small = __half2float(__float2half_rn(y[i] * 0.0625f));
-                        y[i] = small;
-                        sum += small * 16.f;
-                    } else {
-                        sum += y[i];
-                    }
+                    const float unit = (i & 1) ? 0.0625f : 1.f;
+                    y[i] = __half2float(__float2half_rn(f[8 * w + i] * down * unit));
+                    sum += (i & 1) ? y[i] * 16.f : y[i];
                 }
                 qa[2 * w][x] = Elem<__half>::pack(y[0], y[4]);
                 qa[2 * w][2 + x] = Elem<__half>::pack(y[2], y[6]);
@@ -138,7 +131,7 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             qsum[x] = sum;
-            qscale[x] = __uint_as_float((uint32_t)(127 + e2) << 23) * p.scale_log2;
+            qscale[x] = power_of_two(e2) * p.scale_log2;
         }
         // a row past the context sees nothing, whatever its neighbours see
         const bool odd_rows = __any_sync(0xffffffffu, (row_out[0] >= 0 && last[0] < 0) || (row_out[1] >= 0 && last[1] < 0));

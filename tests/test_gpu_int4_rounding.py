@@ -80,6 +80,36 @@ def test_decode_weights_keep_their_bits(cuda_device, dtype, dim, select, heads, 
     assert_rounded_once(actual, expected, float(vals.max() - vals.min()) * 2.0 ** -17, dtype)
 
 
+@pytest.mark.parametrize("dtype,top,small", [
+    # next to a largest element of 1024, two odd elements of 2^-4 that differ by 2^-9 of themselves
+    (torch.float16, 1024.0, (1 + 33 / 1024, 1 + 31 / 1024)),
+    (torch.bfloat16, 8192.0, (1 + 9 / 128, 1 + 7 / 128))])
+@pytest.mark.parametrize("prefill", [False, True])
+def test_small_query_elements_keep_their_bits(cuda_device, dtype, top, small, prefill):
+    gen = np.random.default_rng(2)
+    bs, dim = 16, 64
+    keys, vals = torch.zeros(16, 1, dim), randn(gen, 16, 1, dim)
+    keys[0, 0, 1] = keys[1, 0, 3] = 8192.0
+    kp, vp = pool_of(keys, bs), pool_of(vals, bs)
+    keys, vals = int4_kv.values(kp, bs, dim), int4_kv.values(vp, bs, dim)
+    q = torch.zeros(1, 1, dim)
+    q[0, 0, 0], q[0, 0, 1], q[0, 0, 3] = top, small[0] / 16, small[1] / 16
+    assert torch.equal(q.to(dtype).float(), q)
+    q = q.to(dtype)
+    pools = [torch.from_numpy(p).cuda() for p in (kp, vp)]
+    table, lens = torch.tensor([[0]]), torch.tensor([2])
+    if prefill:
+        meta = torch.tensor([0, 1]), torch.tensor([1]), table, lens
+        expected = int4_kv.paged_prefill(q, keys, vals, *meta, bs)
+        actual = paged_prefill_attention_int4(q.cuda(), *pools, *(m.cuda() for m in meta), bs)
+    else:
+        expected = int4_kv.paged_decode(q, keys, vals, table, lens, bs)
+        actual = paged_attention_int4(q.cuda(), *pools, table.cuda(), lens.cuda(), bs)
+    spread = float(vals[0, :2].max() - vals[0, :2].min())
+    ds = (dim + 8) * 2.0 ** -23 * float(keys.max()) * small[0] / 16 * math.log2(math.e) / math.sqrt(dim)
+    assert_rounded_once(actual, expected, spread * (2.0 ** -17 + 2 * math.log(2) * ds), dtype)
+
+
 def test_prefill_does_not_depend_on_its_neighbours(cuda_device):
     """bf16: a request alone, in batches of short and of long chunks, and on a wider table gives the same bytes."""
     gen = np.random.default_rng(8)
