@@ -10,8 +10,9 @@
 // staged words (fp16 subnormals c 2^-24, c 2^-20; Q of the latter is scaled by
 // 1/16 beforehand, so one accumulator serves both).  P step' is scaled by the
 // power of two above the largest step met so far (raising it rescales O), so
-// that it stays in fp16's normal range whatever the steps are, and rounded to
-// fp16 once: 2^-12 next to the output's own 2^-12 (fp16) or 2^-9 (bf16).
+// that it stays in fp16's normal range whatever the steps are, and enters in
+// two fp16 terms (2^-22): one (2^-12) would move half of an fp16 output's
+// roundings to the next value, and a twentieth of a bf16 one's.
 //
 // Bound by the tensor pipe and by issue: a warp makes its operands from the
 // codes itself.  mma.sync rather than tcgen05: a tcgen05 operand has to lie in
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
             const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
             for (int j = 0; j < NT; j += 2) {
-                uint32_t a[4];
+                uint32_t a[4], a2[4];
 #pragma unroll
                 for (int jj = 0; jj < 2; ++jj) {
                     float2 f[2];  // V step, V base of the two keys
@@ -332,7 +333,10 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
                             z[x] = fmaf(e, f[y].y, z[x]);
                             w[y] = e * f[y].x;
                         }
+                        float back[2];
                         a[2 * jj + x] = Elem<__half>::pack(w[0], w[1]);
+                        Elem<__half>::unpack(a[2 * jj + x], back);
+                        a2[2 * jj + x] = Elem<__half>::pack(w[0] - back[0], w[1] - back[1]);
                     }
                 }
                 const unsigned char* v = st + (BN + 8 * j + q4) * RB + g * (RB / 8);
@@ -376,10 +380,16 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
                     // even nibbles, and whole bytes for the odd ones (as the decode)
                     const uint32_t l0 = x0[u] & 0x00ff00ffu, l1 = x1[u] & 0x00ff00ffu;
                     const uint32_t h0 = permute_bytes(x0[u], 0u, 0x4341u), h1 = permute_bytes(x1[u], 0u, 0x4341u);
-                    mma16816<__half>(o[u][0], a, l0 & kNibbleMask, l1 & kNibbleMask);
+                    const uint32_t m0 = l0 & kNibbleMask, m1 = l1 & kNibbleMask;
+                    const uint32_t n0 = h0 & kNibbleMask, n1 = h1 & kNibbleMask;
+                    mma16816<__half>(o[u][0], a, m0, m1);
                     mma16816<__half>(o[u][1], a, l0, l1);
-                    mma16816<__half>(o[u][2], a, h0 & kNibbleMask, h1 & kNibbleMask);
+                    mma16816<__half>(o[u][2], a, n0, n1);
                     mma16816<__half>(o[u][3], a, h0, h1);
+                    mma16816<__half>(o[u][0], a2, m0, m1);
+                    mma16816<__half>(o[u][1], a2, l0, l1);
+                    mma16816<__half>(o[u][2], a2, n0, n1);
+                    mma16816<__half>(o[u][3], a2, h0, h1);
                 }
             }
         }

@@ -80,6 +80,22 @@ def test_decode_weights_keep_their_bits(cuda_device, dtype, dim, select, heads, 
     assert_rounded_once(actual, expected, float(vals.max() - vals.min()) * 2.0 ** -17, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,heads,count", [(32, 2, 9), (64, 4, 200), (128, 4, 20), (128, 4, 200), (256, 2, 30)])
+def test_prefill_weights_keep_their_bits(cuda_device, dtype, dim, heads, count):
+    gen = np.random.default_rng(dim + count)
+    bs, kv_heads, start = 16, 2, 3
+    rows = -(-(start + count) // bs) * bs, kv_heads, dim
+    kp, vp = pool_of(keys_of_one_value(gen, *rows), bs), pool_of(rows_of_many_steps(gen, *rows), bs)
+    keys, vals = int4_kv.values(kp, bs, dim), int4_kv.values(vp, bs, dim)
+    q = torch.full((count, heads, dim), 0.125, dtype=dtype)
+    meta = torch.tensor([0, count]), torch.tensor([start]), torch.arange(len(kp))[None], torch.tensor([start + count])
+    expected = int4_kv.paged_prefill(q, keys, vals, *meta, bs)
+    actual = paged_prefill_attention_int4(q.cuda(), *(torch.from_numpy(p).cuda() for p in (kp, vp)),
+                                          *(m.cuda() for m in meta), bs)
+    assert_rounded_once(actual, expected, float(vals.max() - vals.min()) * 2.0 ** -17, dtype)
+
+
 @pytest.mark.parametrize("dtype,top,small", [
     # next to a largest element of 1024, two odd elements of 2^-4 that differ by 2^-9 of themselves
     (torch.float16, 1024.0, (1 + 33 / 1024, 1 + 31 / 1024)),
