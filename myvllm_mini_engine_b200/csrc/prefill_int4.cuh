@@ -4,15 +4,16 @@
 // keys [0, start + i] of r's pages (history and current chunk, already written).
 // A CTA takes 64 rows, (token, query head) pairs of one request and kv head, 16
 // a warp, and goes over the keys BN at a time with a running maximum and sum:
-//   S = Q K^T,  s = (step (q . c) + base sum(q)) / sqrt(D),  P = 2^(s - max)
-//   O += (P step') C'^T,  z += P base',  out = (O + z) / sum P
+//   S = Q K^T,  s = (step (q . c) + base sum(q)) / sqrt(D),  P' = 2^(s + log2 step' - max)
+//   O += P' C'^T,  l += P' / step',  z += P' base' / step',  out = (O + z) / l
 // As in decode_pages.cuh the codes are the operands, nibbles masked out of the
 // staged words (fp16 subnormals c 2^-24, c 2^-20; Q of the latter is scaled by
-// 1/16 beforehand, so one accumulator serves both).  P step' is scaled by the
-// power of two above the largest step met so far (raising it rescales O), so
-// that it stays in fp16's normal range whatever the steps are, and enters in
-// two fp16 terms (2^-22): one (2^-12) would move half of an fp16 output's
-// roundings to the next value, and a twentieth of a bf16 one's.
+// 1/16 beforehand, so one accumulator serves both).  The maximum is a
+// row's own, of s + log2 step' over the keys that it sees: keys of no weight, or
+// behind the row, do not move what its P' is rounded to, whatever their steps.
+// P' enters in two fp16 terms (2^-22): one (2^-12) would move half of an fp16
+// output's roundings to the next value, and a twentieth of a bf16 one's (4 x 1000
+// tokens behind 4096, 32/8 heads of 128: 1181 us with one term, 1515 with two).
 //
 // Bound by the tensor pipe and by issue: a warp makes its operands from the
 // codes itself.  mma.sync rather than tcgen05: a tcgen05 operand has to lie in
@@ -55,9 +56,11 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
     __shared__ int64_t row_at[2][BN];     // byte of a key's codes in the pool, or -1
     __shared__ int64_t pair_at[2][BN];
     __shared__ uint32_t valid_s[kPrefillStages][2];
-    // of the keys of a tile, by each warp for itself: K step 2^24, K base, V step, V base
+    // of the keys of a tile, by each warp for itself: K step 2^24, K base, log2 V step, 1 / V step; V base / V step
     __shared__ float4 factors_s[kPrefillWarps][BN];
+    __shared__ float weights_s[kPrefillWarps][BN];
     float4* factors = factors_s[warp];
+    float* weights = weights_s[warp];
     const int kvh = blockIdx.x, r = blockIdx.z;
     griddep_wait();
     griddep_launch_dependents();
@@ -204,7 +207,6 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[u][n][i] = 0.f;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, z[2] = {0.f, 0.f};
-        int vexp = -26;  // steps so far are below 2^(vexp + 1)
 
         for (int kt = 0; kt < nk; ++kt) {
             copy_wait<1>();
@@ -215,20 +217,14 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
             const uint64_t valid = valid_s[kt % kPrefillStages][0] |
                                    (BN > 32 ? (uint64_t)valid_s[kt % kPrefillStages][1] << 32 : 0ull);
             const __half2* pairs = reinterpret_cast<const __half2*>(st + 2 * BN * RB);
-            float vmax = 0.f;
 #pragma unroll
             for (int i = 0; i < BN / 32; ++i) {
                 const float2 k = __half22float2(pairs[32 * i + lane]), v = __half22float2(pairs[BN + 32 * i + lane]);
                 const float vstep = fmaxf(v.x, kInt4StepMin);
-                vmax = fmaxf(vmax, vstep);
-                factors[32 * i + lane] = make_float4(fmaxf(k.x, kInt4StepMin) * kCodeScale, k.y, vstep, v.y);
+                const float inv = rcp_fast(vstep);
+                factors[32 * i + lane] = make_float4(fmaxf(k.x, kInt4StepMin) * kCodeScale, k.y, log2_fast(vstep), inv);
+                weights[32 * i + lane] = v.y * inv;
             }
-            // the largest step's exponent; O's unit is raised when it exceeds the one in use
-            const int ve = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(vmax)) >> 23) - 127;
-            const int raise = max(0, ve - vexp);
-            vexp += raise;
-            const float shrink = raise > 100 ? 0.f : __uint_as_float((uint32_t)(127 - raise) << 23);
-            const float vinv = __uint_as_float((uint32_t)(127 - vexp - 1) << 23);
             __syncwarp();
             // ---- S: column c of key group j is its key c / 2 + 4 (c % 2)
             float s[NT][4];
@@ -268,11 +264,11 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
-                    const float2 f = *reinterpret_cast<const float2*>(&factors[8 * j + q4 + 4 * y]);
+                    const float4 f = factors[8 * j + q4 + 4 * y];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         float& e = s[j][2 * x + y];
-                        e = fmaf(e, f.x, f.y * qsum[x]);
+                        e = fmaf(fmaf(e, f.x, f.y * qsum[x]), qscale[x], f.z);
                     }
                 }
             if (odd_rows || (kt + 1) * BN > warp_near || valid != (BN == 64 ? ~0ull : 0xffffffffull)) {
@@ -288,20 +284,17 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], s[j][i]);
-            const bool higher = mx[0] * qscale[0] > m[0] + kMaxSlack || mx[1] * qscale[1] > m[1] + kMaxSlack;
-            if (__any_sync(0xffffffffu, higher || raise != 0)) {
+            if (__any_sync(0xffffffffu, mx[0] > m[0] + kMaxSlack || mx[1] > m[1] + kMaxSlack)) {
                 float alpha[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
                     mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-                    const float top = mx[x] * qscale[x];
-                    const float mn = top > m[x] + kMaxSlack ? top : m[x];
+                    const float mn = mx[x] > m[x] + kMaxSlack ? mx[x] : m[x];
                     alpha[x] = mn == -INFINITY ? 1.f : exp2_fast(m[x] - mn);
                     m[x] = mn;
                     l[x] *= alpha[x];
                     z[x] *= alpha[x];
-                    alpha[x] *= shrink;
                 }
 #pragma unroll
                 for (int u = 0; u < NW; ++u)
@@ -310,28 +303,27 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
 #pragma unroll
                         for (int i = 0; i < 4; ++i) o[u][n][i] *= alpha[i >> 1];
             }
-            // ---- P, and P step' as the A operand; O, 16 keys at a time
+            // ---- P' as the A operand; O, 16 keys at a time
             const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
             for (int j = 0; j < NT; j += 2) {
                 uint32_t a[4], a2[4];
 #pragma unroll
                 for (int jj = 0; jj < 2; ++jj) {
-                    float2 f[2];  // V step, V base of the two keys
+                    float inv[2], base[2];  // of the two keys: 1 / V step, V base / V step
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        f[y] = *reinterpret_cast<const float2*>(&factors[8 * (j + jj) + q4 + 4 * y].z);
-                        f[y].x *= vinv;
+                        inv[y] = factors[8 * (j + jj) + q4 + 4 * y].w;
+                        base[y] = weights[8 * (j + jj) + q4 + 4 * y];
                     }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         float w[2];
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
-                            const float e = exp2_fast(fmaf(s[j + jj][2 * x + y], qscale[x], -mm[x]));
-                            l[x] += e;
-                            z[x] = fmaf(e, f[y].y, z[x]);
-                            w[y] = e * f[y].x;
+                            w[y] = exp2_fast(s[j + jj][2 * x + y] - mm[x]);
+                            l[x] = fmaf(w[y], inv[y], l[x]);
+                            z[x] = fmaf(w[y], base[y], z[x]);
                         }
                         float back[2];
                         a[2 * jj + x] = Elem<__half>::pack(w[0], w[1]);
@@ -404,17 +396,15 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
             Z += __shfl_xor_sync(0xffffffffu, Z, 2);
             if (row_out[x] < 0) continue;  // no shuffle of this row follows
             const float inv = L == 0.f ? 0.f : 1.f / L;
-            // codes 2^-24, steps 2^-(vexp + 1): the exponent lies in [-1, 40]
-            const float up = __uint_as_float((uint32_t)(127 + vexp + 1 + 24) << 23);
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
                 T* dst = out + row_out[x] + (2 * q4 + y) * (D / 8);
 #pragma unroll
                 for (int u = 0; u < NW; ++u) {
                     const int i = 2 * x + y;
-                    const float f0 = fmaf(o[u][0][i], up, Z) * inv, f2 = fmaf(o[u][2][i], up, Z) * inv;
-                    const float f1 = fmaf(o[u][1][i] - o[u][0][i], up * 0.0625f, Z) * inv;
-                    const float f3 = fmaf(o[u][3][i] - o[u][2][i], up * 0.0625f, Z) * inv;
+                    const float f0 = fmaf(o[u][0][i], kCodeScale, Z) * inv, f2 = fmaf(o[u][2][i], kCodeScale, Z) * inv;
+                    const float f1 = fmaf(o[u][1][i] - o[u][0][i], kCodeScale * 0.0625f, Z) * inv;
+                    const float f3 = fmaf(o[u][3][i] - o[u][2][i], kCodeScale * 0.0625f, Z) * inv;
                     *reinterpret_cast<uint2*>(dst + 4 * u) = make_uint2(Elem<T>::pack(f0, f1), Elem<T>::pack(f2, f3));
                 }
             }

@@ -126,6 +126,34 @@ def test_small_query_elements_keep_their_bits(cuda_device, dtype, top, small, pr
     assert_rounded_once(actual, expected, spread * (2.0 ** -17 + 2 * math.log(2) * ds), dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prefill_rows_do_not_feel_a_value_they_do_not_weigh(cuda_device, dtype):
+    """One value row 2^22 times the others': behind it, for the rows before; of no weight, for the rows after."""
+    gen = np.random.default_rng(6)
+    bs, dim, n, at = 16, 64, 64, 40
+    keys, vals = randn(gen, n, 1, dim), randn(gen, n, 1, dim) * 2.0 ** -9
+    keys[at] = -40.0  # with queries of 0.5: a score of -160
+    q = torch.full((n, 1, dim), 0.5, dtype=dtype)
+    meta = torch.tensor([0, n]), torch.tensor([0]), torch.arange(n // bs)[None], torch.tensor([n])
+    large = vals.clone()
+    large[at] = randn(gen, 1, dim) * 2.0 ** 13
+    kp, vp, lp = pool_of(keys, bs), pool_of(vals, bs), pool_of(large, bs)
+
+    def run(vp):
+        return paged_prefill_attention_int4(q.cuda(), torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(),
+                                            *(m.cuda() for m in meta), bs).cpu()
+
+    without, actual = run(vp), run(lp)
+    assert torch.equal(actual[:at], without[:at])
+    k, v = int4_kv.values(kp, bs, dim), int4_kv.values(lp, bs, dim)
+    expected = int4_kv.paged_prefill(q, k, v, *meta, bs)
+    others = vals[torch.arange(n) != at]
+    spread = float(others.max() - others.min())
+    terms = 2 * dim * 0.5 * float(k.abs().max())
+    ds = (dim + 8) * 2.0 ** -23 * terms * math.log2(math.e) / math.sqrt(dim)
+    assert_rounded_once(actual[at + 1:], expected[at + 1:], spread * (2.0 ** -17 + 2 * math.log(2) * ds), dtype)
+
+
 def test_prefill_does_not_depend_on_its_neighbours(cuda_device):
     """bf16: a request alone, in batches of short and of long chunks, and on a wider table gives the same bytes."""
     gen = np.random.default_rng(8)
