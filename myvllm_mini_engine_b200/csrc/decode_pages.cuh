@@ -11,8 +11,8 @@
 // own: a nibble left in the low bits of a half is the fp16 subnormal c 2^-24
 // (c 2^-20 for the high nibbles), so a mask makes an operand register and the
 // powers of two are taken out of the fp32 results.  The running maximum is that
-// of log2 P' = s + log2(step'), so P' <= 1 is what is rounded to fp16, whatever
-// the steps are; P = P' / step' stays in fp32.
+// of log2 P' = s + log2(step'), so that P' fits fp16 whatever the steps are; P =
+// P' / step' stays in fp32.
 //
 // Split.  A unit is (request, kv head, up to 8 of its query heads).  The tiles
 // (TT tokens) of all units form one list, cut into equal runs, one per CTA of a
@@ -133,10 +133,13 @@ __device__ __forceinline__ float column_sum(float x) {
     return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
 
-// The running maximum is raised only when a score exceeds it by more than 2^8, so P <= 2^8 (fp16
-// holds 65504), O is rescaled once or twice a unit, and the maximum over a column's lanes is taken
-// only then: a vote tells.
-constexpr float kMaxSlack = 8.f;
+// m, which the exponents are taken against, lies kHeadroom below the running maximum (log2), so that P
+// uses fp16's range (65504) and not only its part below 1: a token keeps all bits of P down to 2^-26 of
+// the largest, and is lost below 2^-37 of it, so that a million tokens lose 2^-17 of the weight at most
+// (with the maximum at 1, 2^-25 and 2^-5).  m is raised only when a score exceeds the maximum that it was
+// made for by more than 2^3: P <= 2^15, O is rescaled once or twice a unit, and the maximum over a
+// column's lanes is taken only then: a vote tells.
+constexpr float kHeadroom = 12.f, kMost = 15.f;
 
 // The fp16 query of a 4-bit pool is scaled by a power of two so that a row's largest element lies in
 // [2^14, 2^15): elements keep all of their bits down to 2^-24 of the largest (odd ones, stored 16 times
@@ -153,7 +156,7 @@ constexpr uint32_t kNibbleMask = 0x000f000fu;  // the low nibbles of two halves
 constexpr float kCodeScale = 16777216.f;       // 2^24: a nibble in the low bits of a half is code 2^-24
 
 // ---------------------------------------------------------------- consumers
-// Both keep, per warp: m (running maximum, log2), l (lane's part of sum P),
+// Both keep, per warp: m (kHeadroom below the running maximum, log2), l (lane's part of sum P),
 // z (4-bit: lane's part of sum P base'), o (accumulators) of the unit's query
 // heads; lane (g, q4) = (lane / 4, lane % 4) holds columns (heads) 2 q4, 2 q4 + 1.
 
@@ -307,9 +310,9 @@ struct Int4Consumer {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const float mx = column_max(top[h]);
-            if (mx > m[h] + kMaxSlack) {
-                const float alpha = exp2_fast(m[h] - mx);
-                m[h] = mx;
+            if (mx > m[h] + kMost) {
+                const float alpha = exp2_fast(m[h] - (mx - kHeadroom));
+                m[h] = mx - kHeadroom;
                 l[h] *= alpha;
                 z[h] *= alpha;
 #pragma unroll
@@ -369,7 +372,7 @@ struct Int4Consumer {
         float top[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(t[0][h], t[0][h + 2]), fmaxf(t[1][h], t[1][h + 2]));
-        if (__any_sync(0xffffffffu, top[0] > m[0] + kMaxSlack || top[1] > m[1] + kMaxSlack)) raise(top);
+        if (__any_sync(0xffffffffu, top[0] > m[0] + kMost || top[1] > m[1] + kMost)) raise(top);
         const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};  // 2^(-inf - 0) = 0
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -488,9 +491,9 @@ struct Wide16Consumer {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const float mx = column_max(top[h]);
-            if (mx > m[h] + kMaxSlack) {
-                const float alpha = exp2_fast(m[h] - mx);
-                m[h] = mx;
+            if (mx > m[h] + kMost) {
+                const float alpha = exp2_fast(m[h] - (mx - kHeadroom));
+                m[h] = mx - kHeadroom;
                 l[h] *= alpha;
 #pragma unroll
                 for (int x = 0; x < KSTEPS; ++x) {
@@ -516,7 +519,7 @@ struct Wide16Consumer {
         s[2] = ok1 ? (s[2] + s2[2]) * scale_log2 : -INFINITY;
         s[3] = ok1 ? (s[3] + s2[3]) * scale_log2 : -INFINITY;
         const float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
-        if (__any_sync(0xffffffffu, top[0] > m[0] + kMaxSlack || top[1] > m[1] + kMaxSlack)) raise(top);
+        if (__any_sync(0xffffffffu, top[0] > m[0] + kMost || top[1] > m[1] + kMost)) raise(top);
         const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};  // 2^(-inf - 0) = 0
         float p[4];
 #pragma unroll

@@ -284,13 +284,13 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], s[j][i]);
-            if (__any_sync(0xffffffffu, mx[0] > m[0] + kMaxSlack || mx[1] > m[1] + kMaxSlack)) {
+            if (__any_sync(0xffffffffu, mx[0] > m[0] + kMost || mx[1] > m[1] + kMost)) {
                 float alpha[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
                     mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-                    const float mn = mx[x] > m[x] + kMaxSlack ? mx[x] : m[x];
+                    const float mn = mx[x] > m[x] + kMost ? mx[x] - kHeadroom : m[x];
                     alpha[x] = mn == -INFINITY ? 1.f : exp2_fast(m[x] - mn);
                     m[x] = mn;
                     l[x] *= alpha[x];

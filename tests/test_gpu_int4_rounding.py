@@ -154,6 +154,49 @@ def test_prefill_rows_do_not_feel_a_value_they_do_not_weigh(cuda_device, dtype):
     assert_rounded_once(actual[at + 1:], expected[at + 1:], spread * (2.0 ** -17 + 2 * math.log(2) * ds), dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("form", ["decode", "prefill", "selected"])
+def test_many_light_tokens_keep_their_values(cuda_device, dtype, form):
+    """One token takes the weight; 131071 others, 2^-25.05 of it each, alone have values in the odd dims.
+
+    Those dims hold the light tokens' sum, 2^-8 of their value, on two pages that the table repeats.  P' of a light
+    token keeps 2^-11 at least (fp16, of which it is above the subnormals); the sum of the weights may miss the light
+    ones, 2^-8 (a term below half a step of the sum it is added to).
+    """
+    bs, dim, n = 256, 64, 131072
+    batch, kv_heads = (1, 1) if form == "prefill" else (64, 8)  # so that a warp of a decode has many of the tokens
+    keys, vals = torch.zeros(2 * bs, kv_heads, dim), torch.ones(2 * bs, kv_heads, dim) * 15
+    vals[:, :, 0] = 0.0  # base 0, step 1, codes 0 and 15
+    keys[0] = 25.05 / (math.log2(math.e) * math.sqrt(dim))
+    vals[0, :, 1::2] = 0.0
+    table = torch.ones(batch, n // bs, dtype=torch.int64)
+    table[:, 0] = 0
+    lens = torch.full((batch,), n)
+    q = torch.ones(batch, kv_heads, dim, dtype=dtype)
+    if form == "selected":
+        k16, v16 = (x.view(2, bs, kv_heads, dim).to(dtype) for x in (keys, vals))
+        k, v = k16.double(), v16.double()
+        listed = torch.arange(n // bs).expand(batch, kv_heads, -1).contiguous()
+        actual = paged_attention_selected(q.cuda(), k16.cuda(), v16.cuda(), table.cuda(), lens.cuda(), listed.cuda(), bs)
+    else:
+        kp, vp = pool_of(keys, bs), pool_of(vals, bs)
+        k, v = int4_kv.values(kp, bs, dim), int4_kv.values(vp, bs, dim)
+        pools = [torch.from_numpy(p).cuda() for p in (kp, vp)]
+        if form == "decode":
+            actual = paged_attention_int4(q.cuda(), *pools, table.cuda(), lens.cuda(), bs)
+        else:
+            meta = torch.tensor([0, 1]), torch.tensor([n - 1]), table, lens
+            actual = paged_prefill_attention_int4(q.cuda(), *pools, *(m.cuda() for m in meta), bs)
+    weight = torch.exp(float(k[0, 0, 0].sum()) / math.sqrt(dim) * torch.tensor([1.0, 0.0], dtype=torch.float64))
+    weight[1] *= n - 1
+    weight /= weight.sum()
+    odd = (weight[0] * v[0, 0, 0] + weight[1] * v[1, 0, 0])[1::2].expand(batch, kv_heads, -1)
+    assert 0.02 < float(odd.min()) < 0.1
+    ds = (dim + 8) * 2.0 ** -23 * 25.05
+    bound = half_step(odd, dtype) + odd * (2.0 ** -7.9 + 2.0 ** -11 + 2 * math.log(2) * ds)
+    assert bool(((actual.double().cpu()[..., 1::2] - odd).abs() <= bound).all()), actual[0, 0, :8]
+
+
 def test_prefill_does_not_depend_on_its_neighbours(cuda_device):
     """bf16: a request alone, in batches of short and of long chunks, and on a wider table gives the same bytes."""
     gen = np.random.default_rng(8)
