@@ -302,8 +302,10 @@ int minikv_paged_prefill(const void* q, const void* key_cache, const void* value
  * 2^-24.  A row (one token, one kv head, K or V) is quantised by itself:
  *   base = fp16(min), step = fp16(max(2^-24, (max - min) / 15)),
  *   code = round((x - base) / step) clamped to 0..15 (nearest even),
- * with NaN counted as 0 and magnitudes saturated at 65504.  head_dim in {32,
- * 64, 96, 128, 192, 256}; any block_size.  Returns -1 for other shapes. */
+ * with NaN counted as 0 and magnitudes saturated at 65504; where base + 15 step
+ * would pass 65504, step is the largest fp16 (2^-24 at least) with which it does
+ * not, so that a row written reads as finite fp16.  head_dim in {32, 64, 96, 128,
+ * 192, 256}; any block_size.  Returns -1 for other shapes. */
 int64_t minikv_int4_page_bytes(int64_t block_size, int64_t head_dim);
 
 /* Quantising writes from fp32/fp16/bf16 rows, with the destinations of

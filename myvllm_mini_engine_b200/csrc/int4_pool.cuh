@@ -7,7 +7,9 @@
 // below 2^-24 reads as 2^-24.  A row (one token, one kv head, K or V) is
 // quantised by itself: base = fp16(min), step = fp16(max(2^-24, (max - min) / 15)),
 // code = round((x - base) / step) clamped to 0..15 (true quotients, nearest
-// even).  NaN counts as 0 and magnitudes saturate at 65504.  At D = 128 a row
+// even).  NaN counts as 0 and magnitudes saturate at 65504; where base + 15 step
+// would pass it, the step is the largest fp16 with which it does not (2^-24 at
+// least): every element then reads as a finite fp16.  At D = 128 a row
 // takes 68 bytes, 4.25 bits an element, against 256 in a 16-bit pool.  One
 // pair per row (not per smaller group) lets the attention fold the key's step
 // into the score and the value's step into the probability, so that the codes
@@ -103,6 +105,14 @@ template <typename T, bool VEC> struct RowPart {
     }
 };
 
+// The step of a row from lo to hi whose base is b.
+__device__ __forceinline__ __half int4_step(float lo, float hi, float b) {
+    __half step = __float2half_rn(fmaxf(__fdiv_rn(hi - lo, 15.f), kInt4StepMin));
+    if (__fadd_rn(b, 15.f * __half2float(step)) > 65504.f)  // rare: rows that end near 65504
+        step = __float2half_rd(fmaxf(__fdiv_rd(__fsub_rd(65504.f, b), 15.f), kInt4StepMin));
+    return step;
+}
+
 // Code of one element by the format's own words.
 __device__ __forceinline__ uint32_t int4_code(float x, float base, float step) {
     return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x - base, step)), 0.f), 15.f);
@@ -183,8 +193,9 @@ __global__ void __launch_bounds__(256, kInt4WriteBlocks) int4_write_kernel(
         }
         if (row < 0) continue;  // no shuffle follows in this iteration
         const __half base = __float2half_rn(lo);
-        const __half step = __float2half_rn(fmaxf(__fdiv_rn(hi - lo, 15.f), kInt4StepMin));
-        const float b = __half2float(base), s = __half2float(step);
+        const float b = __half2float(base);
+        const __half step = int4_step(lo, hi, b);
+        const float s = __half2float(step);
         float inv;  // 1 / s within 2^-22
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
         const uint32_t page = block_of((uint32_t)row), off_in = (uint32_t)row - page * block_of.d;

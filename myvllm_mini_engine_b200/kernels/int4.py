@@ -13,7 +13,8 @@ of byte i), then ``block_size`` pairs of fp16 (step, base), padded to 16 bytes.
 Element ``x`` of a row is stored as ``code = round((x - base) / step)`` in 0..15
 with ``base = fp16(min)`` and ``step = fp16(max(2^-24, (max - min) / 15))`` of its
 row (one token, one kv head, K or V by itself), and read as ``base + step * code``.
-NaN counts as 0 and magnitudes saturate at 65504.  At head_dim 128 that is 4.25
+NaN counts as 0 and magnitudes saturate at 65504; the step is rounded down where
+``base + 15 * step`` would pass that.  At head_dim 128 that is 4.25
 bits an element: a decode step streams 68 bytes where a 16-bit pool has 256.
 
 The decode's scratch memory is kept per stream for eager calls; a captured call

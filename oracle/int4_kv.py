@@ -27,6 +27,13 @@ def quantize(x):
     low, high = x.min(-1, keepdims=True), x.max(-1, keepdims=True)
     base = low.astype(np.float16)
     step = np.maximum((high - low) / np.float32(15), STEP_MIN).astype(np.float16)
+    # base + 15 step stays within 65504: else the largest fp16 with which it does (the step's least at least)
+    wide = base.astype(np.float64)
+    most = np.maximum((65504 - wide) / 15, float(STEP_MIN))
+    down = most.astype(np.float16)
+    down = np.where(down.astype(np.float64) > most, np.nextafter(down, np.float16(0)), down)
+    over = (base.astype(np.float32) + np.float32(15) * step.astype(np.float32)) > np.float32(65504)
+    step = np.where(over, down, step)
     d = x - base.astype(np.float32)
     codes = np.clip(np.rint(d / step.astype(np.float32)), 0, 15).astype(np.uint8)
     return codes, step[..., 0], base[..., 0]

@@ -219,3 +219,42 @@ def test_prefill_does_not_depend_on_its_neighbours(cuda_device):
     alone = run([count], [start], 7)
     for counts, starts, width in (([count, 1, 1], [start, 5, 90], 7), ([count, 200], [start, 11], 14), ([count], [start], 60000)):
         assert torch.equal(run(counts, starts, width), alone)
+
+
+def saturating_rows(gen, dim):
+    """Rows whose largest element, or what it is rounded to, lies at the end of fp16's range (65504)."""
+    x = randn(gen, 24, 2, dim) * torch.tensor([3e4, 2e4, 1.0])[torch.arange(24) % 3][:, None, None]
+    x[0, 0, 0], x[0, 0, 1] = -65504.0, 65504.0   # step 8733.87, nearest fp16 8736: 15 of them reach 65536
+    x[3, 0, 2], x[6, 1, 5], x[6, 1, 6] = math.inf, -math.inf, 1e30
+    x[9] = -50.0
+    x[9, :, 7] = 65504.0                          # step 4370.27, nearest 4372: 65530
+    x[12], x[15] = 65504.0, 65500.0               # constant rows
+    x[18], x[18, :, 3] = 65504.0, 65489.0         # the least element rounds up to the largest
+    x[21], x[21, :, 0] = 60010.0, 65504.0
+    return x
+
+
+@pytest.mark.parametrize("src", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim", [32, 96, 128])
+def test_rows_at_the_end_of_the_range_read_back_finite(cuda_device, src, dim):
+    from myvllm_mini_engine_b200.kernels import read_kv_cache_slots_int4, write_kv_cache_slots_int4
+
+    bs = 16
+    x = saturating_rows(np.random.default_rng(dim), dim).to(src)
+    slots = torch.arange(24)
+    got = torch.zeros(2, 2, 2, int4_page_bytes(bs, dim), dtype=torch.uint8, device="cuda")
+    write_kv_cache_slots_int4(got[0], got[1], slots.cuda(), x.cuda(), x.cuda(), bs)
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        key, value = read_kv_cache_slots_int4(got[0], got[1], slots.cuda(), bs, dim, dtype=dtype)
+        assert bool(torch.isfinite(key).all()) and torch.equal(key, value)
+        if dtype != torch.bfloat16:  # (65504 rounds to 65536 in bf16)
+            assert float(key.abs().max()) <= 65504.0
+    assert np.array_equal(got[0].cpu().numpy(), pool_of(x, bs))
+    assert np.array_equal(got[1].cpu().numpy(), pool_of(x, bs))
+    # an output that is one such value
+    query = torch.zeros(24, 2, dim, dtype=torch.float16)
+    table, lens = torch.arange(2)[None], torch.tensor([1])
+    out = paged_attention_int4(query[:1].cuda(), got[0], got[1], table.cuda(), lens.cuda(), bs)
+    assert bool(torch.isfinite(out).all())
+    meta = torch.tensor([0, 24]), torch.tensor([0]), table, torch.tensor([24])
+    assert bool(torch.isfinite(paged_prefill_attention_int4(query.cuda(), got[0], got[1], *(m.cuda() for m in meta), bs)).all())

@@ -1,8 +1,11 @@
 """What the 4-bit pool promises, as far as it shows without a GPU."""
 
+import numpy as np
 import pytest
+import torch
 
 from myvllm_mini_engine_b200 import _lib
+from oracle import int4_kv
 
 
 @pytest.mark.parametrize("tokens,requests,width", [(1, 1, 1), (2048, 16, 72), (16384, 16, 65536), (200, 16, 65536)])
@@ -13,3 +16,20 @@ def test_a_prefill_takes_no_workspace(tokens, requests, width, dtype):
         size = _lib.load().minikv_paged_prefill_int4_workspace_bytes(tokens, requests, heads, kv_heads, dim, 1 << 20, 16,
                                                                      width, dtype)
         assert size == 0
+
+
+def test_the_oracle_reads_rows_at_the_end_of_the_range_back_finite():
+    """Rows from -65504, and from values that round up, to 65504; half a step of the value away at most."""
+    gen = np.random.default_rng(3)
+    x = torch.from_numpy(gen.uniform(-65504, 65504, (400, 64)).astype(np.float32))
+    x[:, 1] = 65504.0
+    low = torch.from_numpy(gen.uniform(-65504, 65504, 400).astype(np.float32))
+    x = torch.maximum(x, low[:, None])  # rows of every width up to the whole range
+    x[0, 0], x[1], x[2] = -65504.0, 65504.0, 65489.0
+    x[2, 3] = 65504.0
+    codes, step, base = (torch.from_numpy(np.asarray(v, dtype=np.float64)) for v in int4_kv.quantize(x))
+    back = base[:, None] + step[:, None] * codes
+    assert float(back.max()) <= 65504.0 and bool(torch.isfinite(back.half()).all())
+    # half a step; base and step were rounded (2^-11 of base, 2^-10 of 15 steps rounded down)
+    bound = step / 2 + base.abs() * 2.0 ** -11 + 15 * step * 2.0 ** -10
+    assert bool(((back - x.double()).abs() <= bound[:, None]).all())
