@@ -430,9 +430,10 @@ __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) score_blocks_kernel(con
         neg = fmaxf(neg, -kLargest);
         sums[h][d] = pos;
         sums[h][D + d] = neg;
-        // non-negative floats order as their bits
-        const int top = __reduce_max_sync(__activemask(), __float_as_int(fmaxf(pos, -neg)));
-        if (lane == 0) atomicMax(&tops[h], top);  // a warp's 32 dims are of one head
+        // non-negative floats order as their bits; a warp's 32 dims are of one head, and all of its lanes
+        // are here (nh * D is a multiple of 32)
+        const int top = __reduce_max_sync(0xffffffffu, __float_as_int(fmaxf(pos, -neg)));
+        if (lane == 0) atomicMax(&tops[h], top);
     }
     __syncthreads();
     for (int x = tid; x < kScoreHeads * 2 * D; x += 256) {
