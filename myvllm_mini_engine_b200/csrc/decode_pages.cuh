@@ -984,6 +984,7 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 
                 if (lane == 0)
                     asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;"
                                  : "=r"(old) : "l"(p.tickets + unit), "r"((unsigned int)(c1 - c0)) : "memory");
+                __syncwarp();  // and its acquire the loads of the warp behind it (a shuffle orders no memory)
                 if (__shfl_sync(0xffffffffu, old, 0) == (unsigned int)(c1 - c0))
                     join_partials<T, D>(p, unit + c0, c1 - c0 + 1, heads, qh0, lane, 32);
             }

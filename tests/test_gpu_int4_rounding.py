@@ -258,3 +258,25 @@ def test_rows_at_the_end_of_the_range_read_back_finite(cuda_device, src, dim):
     assert bool(torch.isfinite(out).all())
     meta = torch.tensor([0, 24]), torch.tensor([0]), table, torch.tensor([24])
     assert bool(torch.isfinite(paged_prefill_attention_int4(query.cuda(), got[0], got[1], *(m.cuda() for m in meta), bs)).all())
+
+
+@pytest.mark.parametrize("heads", [2, 8])
+def test_warps_that_share_a_unit_join_all_of_its_parts(cuda_device, heads):
+    """Every call gives the 64-bit answer's bytes again: units cut among the warps of several CTAs, many times over."""
+    gen = np.random.default_rng(11)
+    bs, dim, kv_heads, batch, n = 16, 64, 1, 600, 1500
+    rows = 40 * bs, kv_heads, dim
+    kp, vp = pool_of(keys_of_one_value(gen, *rows), bs), pool_of(rows_of_many_steps(gen, *rows), bs)
+    keys, vals = int4_kv.values(kp, bs, dim), int4_kv.values(vp, bs, dim)
+    table = torch.from_numpy(gen.integers(0, 40, (batch, -(-n // bs))).astype(np.int64))
+    lens = torch.from_numpy(gen.integers(n // 2, n, batch).astype(np.int64))
+    warps = torch.cuda.get_device_properties(0).multi_processor_count * 16
+    assert 5 * warps <= int(((lens + 31) // 32).sum()) and -(-n // 32) * warps <= 8 * int(((lens + 31) // 32).sum())
+    query = torch.full((batch, heads, dim), 0.125, dtype=torch.float16)
+    args = query.cuda(), torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda(), table.cuda(), lens.cuda(), bs
+    first = paged_attention_int4(*args)
+    expected = int4_kv.paged_decode(query, keys, vals, table, lens, bs)
+    # (partials: up to ten more sums, and sums of up to 1500 tokens)
+    assert_rounded_once(first, expected, float(vals.max() - vals.min()) * 2.0 ** -15, torch.float16)
+    for _ in range(50):
+        assert torch.equal(paged_attention_int4(*args, validate=False), first)
