@@ -80,8 +80,10 @@ int minikv_set_wait_limit(uint64_t limit_ns, void* stream);
  * captured graph stays valid when lengths change.
  * workspace: device scratch of at least minikv_paged_decode_workspace_bytes()
  * bytes, zero-filled before its first use (e.g. one cudaMemset) and then
- * reused as is: every call leaves the ticket counters it keeps there at zero.
- * Calls that share a workspace must not overlap on the GPU. */
+ * reused as is, by calls of any shape: its first 64 KB hold ticket counters and
+ * nothing else, and every call leaves them at zero (a batch with more counters
+ * than fit there zeroes its own).  Calls that share a workspace must not overlap
+ * on the GPU. */
 int64_t minikv_paged_decode_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                             int64_t head_dim, int64_t num_blocks, int64_t block_size,
                                             int64_t table_width, int dtype);

@@ -146,6 +146,7 @@ int64_t minikv_paged_decode_workspace_bytes(int64_t batch, int64_t q_heads, int6
     DecodePlan plan;
     if (!make_decode_plan(batch, q_heads, kv_heads, head_dim, block_size, table_width, dtype, sm_count(), &plan))
         return -1;
+    keep_tickets_apart(&plan);
     return plan.ws_bytes;
 }
 
@@ -254,6 +255,7 @@ int64_t minikv_paged_decode_fp8_workspace_bytes(int64_t batch, int64_t q_heads, 
     DecodePlan plan;
     if (!make_decode_plan(batch, q_heads, kv_heads, head_dim, block_size, table_width, dtype, sm_count(), &plan, true))
         return -1;
+    keep_tickets_apart(&plan);
     return plan.ws_bytes;
 }
 
@@ -276,6 +278,7 @@ static int run_decode_fp8(const void* query, const void* key_cache, const void* 
     DecodePlan plan;
     if (!make_decode_plan(batch, q_heads, kv_heads, head_dim, block_size, table_width, dtype, sm_count(), &plan, true))
         return fail(MINIKV_EUNSUPPORTED, "decode shape does not fit shared memory (batch too large?)");
+    keep_tickets_apart(&plan);
     MINIKV_REQUIRE(workspace != nullptr && workspace_bytes >= plan.ws_bytes && aligned16(workspace),
                    MINIKV_EINVAL, "decode workspace too small or misaligned");
     DecodeParams p = decode_params(query, key_cache, value_cache, block_tables, lens, nullptr, out,
@@ -293,8 +296,10 @@ static int run_decode_fp8(const void* query, const void* key_cache, const void* 
     }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool e5m2 = fp8_format == MINIKV_FP8_E5M2;
-    const cudaError_t err = dtype == MINIKV_F16 ? launch_decode_fp8<__half>(e5m2, (int)head_dim, p, plan, s)
-                                                : launch_decode_fp8<__nv_bfloat16>(e5m2, (int)head_dim, p, plan, s);
+    cudaError_t err = zero_tickets(plan, workspace, s);
+    if (err == cudaSuccess)
+        err = dtype == MINIKV_F16 ? launch_decode_fp8<__half>(e5m2, (int)head_dim, p, plan, s)
+                                  : launch_decode_fp8<__nv_bfloat16>(e5m2, (int)head_dim, p, plan, s);
     if (err != cudaSuccess) return cuda_fail(err, "minikv_paged_decode_fp8 launch");
     return MINIKV_OK;
 }

@@ -817,6 +817,7 @@ struct DecodePlan {
         head_groups;
     int grid, smem_bytes;
     int64_t records, ws_tickets, ws_lse, ws_partial, ws_bytes;
+    int64_t zero_bytes;  // of the tickets, where the launch has to zero them itself
 };
 
 static int esize_of(int dtype) { return dtype == 0 ? 4 : 2; }
@@ -893,7 +894,27 @@ static bool make_decode_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int6
     plan->ws_lse = align256(B * z * 4);
     plan->ws_partial = plan->ws_lse + align256(plan->records * Hq * 4);
     plan->ws_bytes = plan->ws_partial + align256(plan->records * Hq * D * 4);
+    plan->zero_bytes = 0;
     return true;
+}
+
+// A caller's workspace serves calls of any shape, and nothing but tickets may lie where another call has
+// its own: the first 64 KB are tickets and nothing else, whatever the batch.  A batch that needs more has
+// its tickets behind them, where an earlier call may have left sums, and zeroes them at each call.
+constexpr int64_t kTicketRegion = 64 << 10;
+static void keep_tickets_apart(DecodePlan* plan) {
+    const int64_t tickets = plan->ws_lse;  // their bytes: they come first
+    const bool fits = tickets <= kTicketRegion;
+    const int64_t shift = fits ? kTicketRegion - tickets : kTicketRegion;
+    plan->ws_tickets = fits ? 0 : kTicketRegion;
+    plan->zero_bytes = fits ? 0 : tickets;
+    plan->ws_lse += shift;
+    plan->ws_partial += shift;
+    plan->ws_bytes += shift;
+}
+static cudaError_t zero_tickets(const DecodePlan& plan, void* workspace, cudaStream_t stream) {
+    if (plan.zero_bytes == 0) return cudaSuccess;
+    return cudaMemsetAsync(static_cast<unsigned char*>(workspace) + plan.ws_tickets, 0, (size_t)plan.zero_bytes, stream);
 }
 
 template <typename T, int D>
@@ -976,11 +997,12 @@ static int run_decode(const void* query, const void* key_cache, const void* valu
     DecodePlan plan;
     if (!make_decode_plan(batch, q_heads, kv_heads, head_dim, block_size, table_width, dtype, sm_count(), &plan))
         return fail(MINIKV_EUNSUPPORTED, "decode shape does not fit shared memory (batch too large?)");
+    if (table_rows == nullptr) keep_tickets_apart(&plan);  // (a prefill has a workspace and zeroes for each launch)
     MINIKV_REQUIRE(workspace != nullptr && workspace_bytes >= plan.ws_bytes && aligned16(workspace),
                    MINIKV_EINVAL, "decode workspace too small or misaligned");
     unsigned char* ws = static_cast<unsigned char*>(workspace);
-    // The ticket region (the first bytes of the workspace) must be zero when
-    // the kernel starts; every launch leaves it zero again (atomicInc wraps).
+    // The tickets must be zero when the kernel starts; every launch leaves them
+    // zero again (atomicInc wraps).
     const DecodeParams p = decode_params(query, key_cache, value_cache, block_tables, context_lens, table_rows,
                                          out, ws, batch, q_heads, kv_heads, head_dim, num_blocks, block_size,
                                          table_width, plan);
@@ -992,12 +1014,13 @@ static int run_decode(const void* query, const void* key_cache, const void* valu
         q.new_k = new_k;
         q.new_v = new_v;
     }
-    const cudaError_t err = launch_decode(dtype, (int)head_dim, q, plan, stream);
+    cudaError_t err = zero_tickets(plan, workspace, stream);
+    if (err == cudaSuccess) err = launch_decode(dtype, (int)head_dim, q, plan, stream);
     if (err != cudaSuccess) return cuda_fail(err, "minikv_paged_decode launch");
     return MINIKV_OK;
 }
 
-// Bytes at the start of a decode workspace that must be zero before its first use.
+// Bytes at the start of a workspace laid out by make_decode_plan that must be zero at the launch.
 static int64_t decode_ticket_bytes(const DecodePlan& plan) { return plan.ws_lse; }
 
 }  // namespace minikv

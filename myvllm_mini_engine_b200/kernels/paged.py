@@ -127,8 +127,9 @@ _RETIRED: list = []
 def _workspace(device, stream, need):
     """Zero-filled scratch reused by every decode call on ``stream`` (a raw stream handle).
 
-    The kernel keeps per-request ticket counters in it and leaves them at zero,
-    so it is zeroed once, when allocated.  Calls on one stream never overlap;
+    The kernel keeps ticket counters in its first 64 KB, where calls of every
+    shape keep nothing else, and leaves them at zero, so it is zeroed once, when
+    allocated.  Calls on one stream never overlap;
     each stream gets its own buffer.  Buffers are never freed while the process
     runs, because a captured CUDA graph may still refer to one.
     """
