@@ -83,6 +83,7 @@ class _Pool:
 
     @property
     def memory_bytes(self) -> int:
+        """Bytes of the K and V pages (the block bounds of a pool that has them: ``bounds_bytes``)."""
         return (self.key.numel() + self.value.numel()) * self.key.element_size()
 
     def layer(self, index):
@@ -99,6 +100,11 @@ class _BoundedPool(_Pool):
     """
 
     bounds: torch.Tensor | None = None
+
+    @property
+    def bounds_bytes(self) -> int:
+        """Bytes of the block bounds, 0 without: at head_dim 128 and pages of 16 an eighth of a 4-bit pool's pages."""
+        return 0 if self.bounds is None else self.bounds.numel()
 
     def _make_bounds(self, wanted):
         from ..kernels.sparse import block_bounds_bytes

@@ -33,3 +33,13 @@ def test_the_oracle_reads_rows_at_the_end_of_the_range_back_finite():
     # half a step; base and step were rounded (2^-11 of base, 2^-10 of 15 steps rounded down)
     bound = step / 2 + base.abs() * 2.0 ** -11 + 15 * step * 2.0 ** -10
     assert bool(((back - x.double()).abs() <= bound[:, None]).all())
+
+
+def test_pools_tell_the_bytes_of_their_bounds():
+    from myvllm_mini_engine_b200.cache import INT4KVCachePool, PagedKVPool
+
+    for make, share in ((INT4KVCachePool, 8), (PagedKVPool, 30)):
+        plain, held = (make(2, 5, 16, 3, 128, device="cpu", block_bounds=b) for b in (False, True))
+        assert plain.bounds_bytes == 0 and held.memory_bytes == plain.memory_bytes
+        assert held.bounds_bytes == 2 * 5 * 3 * (2 * 128 + 16) == held.bounds.nbytes
+        assert held.memory_bytes // held.bounds_bytes == share
