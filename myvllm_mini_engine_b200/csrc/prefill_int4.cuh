@@ -46,8 +46,11 @@ constexpr int kPrefillThreads = kPrefillWarps * 32;
 constexpr int kPrefillRows = kPrefillWarps * 16;
 constexpr int kPrefillStages = 3;
 
+// CTAs a SM: three at 64 dims or fewer (4 x 1000 tokens behind 4096, 32/8 heads of 64: 878 us, with two
+// 927); at 96 and 128 the registers of three spill, and two take 1473 against 1500 us at 128, and 32 x 8
+// tokens behind 2048 with 16/8 heads 100 against 152.
 template <typename T, int D>
-__global__ void __launch_bounds__(kPrefillThreads, D <= 128 ? 3 : 2) prefill_int4_kernel(const PrefillInt4Params p) {
+__global__ void __launch_bounds__(kPrefillThreads, D <= 64 ? 3 : 2) prefill_int4_kernel(const PrefillInt4Params p) {
     constexpr int BN = D <= 128 ? 64 : 32;  // keys a tile: the accumulators of S take BN / 2 registers
     constexpr int RB = D / 2, CPR = RB / 16, NW = D / 32, NT = BN / 8;
     constexpr int STAGE = BN * (2 * RB + 8);  // K codes, V codes, K pairs, V pairs
