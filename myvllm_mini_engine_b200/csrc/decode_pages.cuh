@@ -121,6 +121,14 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// d = a b, with nothing added
+__device__ __forceinline__ void mma16816_first(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // max over the 8 lanes that share a column of an accumulator (lanes of equal lane % 4)
 __device__ __forceinline__ float column_max(float x) {
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
@@ -374,6 +382,7 @@ struct Int4Consumer {
         for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(t[0][h], t[0][h + 2]), fmaxf(t[1][h], t[1][h + 2]));
         if (__any_sync(0xffffffffu, top[0] > m[0] + kMost || top[1] > m[1] + kMost)) raise(top);
         const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};  // 2^(-inf - 0) = 0
+        uint32_t w[2][2], w2[2][2];  // P' of a slice, transposed: the terms that this lane's columns multiply
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float p[4];
@@ -390,24 +399,47 @@ struct Int4Consumer {
             const uint32_t r01 = Elem<__half>::pack(p[0] - back[0], p[1] - back[1]);
             const uint32_t r23 = Elem<__half>::pack(p[2] - back[2], p[3] - back[3]);
             const bool second = TWIN && q4 >= 2;
-            uint32_t x0[NH], x1[NH];
-            const unsigned char* v = vst + (16 * i + q4) * RB + g * (RB / 8);
-            load_v(v, v + 4 * RB, x0);
-            load_v(v + 8 * RB, v + 12 * RB, x1);
-            add_values(x0, x1, transpose8x8(second ? r01 : p01), transpose8x8(second ? r23 : p23));
-            if constexpr (!TWIN) add_values(x0, x1, transpose8x8(r01), transpose8x8(r23));
+            w[i][0] = transpose8x8(second ? r01 : p01);
+            w[i][1] = transpose8x8(second ? r23 : p23);
+            if constexpr (!TWIN) {
+                w2[i][0] = transpose8x8(r01);
+                w2[i][1] = transpose8x8(r23);
+            }
         }
-    }
-
-    // O of 16 tokens
-    __device__ __forceinline__ void add_values(const uint32_t* x0, const uint32_t* x1, uint32_t b0, uint32_t b1) {
+        uint32_t x[2][2][NH];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const unsigned char* v = vst + (16 * i + q4) * RB + g * (RB / 8);
+            load_v(v, v + 4 * RB, x[i][0]);
+            load_v(v + 8 * RB, v + 12 * RB, x[i][1]);
+        }
+        // O of the tile by itself, then added: an MMA truncates its sum, which the codes (none negative)
+        // would turn into a bias that grows with the tokens
 #pragma unroll
         for (int u = 0; u < NH; ++u) {
-            const uint32_t b[4] = {x0[u] & 0x00ff00ffu, permute_bytes(x0[u], 0u, 0x4341u), x1[u] & 0x00ff00ffu,
-                                   permute_bytes(x1[u], 0u, 0x4341u)};
-            const uint32_t a[4] = {b[0] & kNibbleMask, b[1] & kNibbleMask, b[2] & kNibbleMask, b[3] & kNibbleMask};
-            mma16816<__half>(o[2 * u], a, b0, b1);
-            mma16816<__half>(o[2 * u + 1], b, b0, b1);
+            float even[4], whole[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t b[4] = {x[i][0][u] & 0x00ff00ffu, permute_bytes(x[i][0][u], 0u, 0x4341u),
+                                       x[i][1][u] & 0x00ff00ffu, permute_bytes(x[i][1][u], 0u, 0x4341u)};
+                const uint32_t a[4] = {b[0] & kNibbleMask, b[1] & kNibbleMask, b[2] & kNibbleMask, b[3] & kNibbleMask};
+                if (i == 0) {
+                    mma16816_first(even, a, w[i][0], w[i][1]);
+                    mma16816_first(whole, b, w[i][0], w[i][1]);
+                } else {
+                    mma16816<__half>(even, a, w[i][0], w[i][1]);
+                    mma16816<__half>(whole, b, w[i][0], w[i][1]);
+                }
+                if constexpr (!TWIN) {
+                    mma16816<__half>(even, a, w2[i][0], w2[i][1]);
+                    mma16816<__half>(whole, b, w2[i][0], w2[i][1]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[2 * u][e] += even[e];
+                o[2 * u + 1][e] += whole[e];
+            }
         }
     }
 

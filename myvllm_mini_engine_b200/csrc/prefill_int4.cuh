@@ -46,6 +46,29 @@ constexpr int kPrefillThreads = kPrefillWarps * 32;
 constexpr int kPrefillRows = kPrefillWarps * 16;
 constexpr int kPrefillStages = 3;
 
+// N (1, 2 or 4) 16-bit runs of the rows of two keys, side by side (the first key's in the low half)
+template <int N>
+__device__ __forceinline__ void load_value_runs(const unsigned char* a, const unsigned char* b, uint32_t* x) {
+    if constexpr (N == 1) {
+        x[0] = *reinterpret_cast<const uint16_t*>(a) | ((uint32_t) * reinterpret_cast<const uint16_t*>(b) << 16);
+    } else {
+        uint32_t wa[N / 2], wb[N / 2];
+        if constexpr (N == 4) {
+            const uint2 c = *reinterpret_cast<const uint2*>(a), d = *reinterpret_cast<const uint2*>(b);
+            wa[0] = c.x; wa[1] = c.y;
+            wb[0] = d.x; wb[1] = d.y;
+        } else {
+            wa[0] = *reinterpret_cast<const uint32_t*>(a);
+            wb[0] = *reinterpret_cast<const uint32_t*>(b);
+        }
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            x[2 * i] = permute_bytes(wa[i], wb[i], 0x5410u);
+            x[2 * i + 1] = permute_bytes(wa[i], wb[i], 0x7632u);
+        }
+    }
+}
+
 // CTAs a SM: three at 64 dims or fewer (4 x 1000 tokens behind 4096, 32/8 heads of 64: 878 us, with two
 // 927); at 96 and 128 the registers of three spill, and two take 1473 against 1500 us at 128, and 32 x 8
 // tokens behind 2048 with 16/8 heads 100 against 152.
@@ -53,6 +76,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kPrefillThreads, D <= 64 ? 3 : 2) prefill_int4_kernel(const PrefillInt4Params p) {
     constexpr int BN = D <= 128 ? 64 : 32;  // keys a tile: the accumulators of S take BN / 2 registers
     constexpr int RB = D / 2, CPR = RB / 16, NW = D / 32, NT = BN / 8;
+    constexpr int NV = NW % 4 == 0 ? 4 : NW % 2 == 0 ? 2 : 1;  // 16-bit runs of V a lane loads at once, of NW (registers)
     constexpr int STAGE = BN * (2 * RB + 8);  // K codes, V codes, K pairs, V pairs
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     __shared__ __align__(128) unsigned char ring[kPrefillStages * STAGE];
@@ -306,86 +330,67 @@ __global__ void __launch_bounds__(kPrefillThreads, D <= 64 ? 3 : 2) prefill_int4
 #pragma unroll
                         for (int i = 0; i < 4; ++i) o[u][n][i] *= alpha[i >> 1];
             }
-            // ---- P' as the A operand; O, 16 keys at a time
+            // ---- P' as the A operands
             const float mm[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+            uint32_t a[NT / 2][4], a2[NT / 2][4];
 #pragma unroll
-            for (int j = 0; j < NT; j += 2) {
-                uint32_t a[4], a2[4];
+            for (int j = 0; j < NT; ++j) {
+                float inv[2], base[2];  // of the two keys: 1 / V step, V base / V step
 #pragma unroll
-                for (int jj = 0; jj < 2; ++jj) {
-                    float inv[2], base[2];  // of the two keys: 1 / V step, V base / V step
+                for (int y = 0; y < 2; ++y) {
+                    inv[y] = factors[8 * j + q4 + 4 * y].w;
+                    base[y] = weights[8 * j + q4 + 4 * y];
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float w[2], back[2];
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        inv[y] = factors[8 * (j + jj) + q4 + 4 * y].w;
-                        base[y] = weights[8 * (j + jj) + q4 + 4 * y];
+                        w[y] = exp2_fast(s[j][2 * x + y] - mm[x]);
+                        l[x] = fmaf(w[y], inv[y], l[x]);
+                        z[x] = fmaf(w[y], base[y], z[x]);
                     }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float w[2];
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            w[y] = exp2_fast(s[j + jj][2 * x + y] - mm[x]);
-                            l[x] = fmaf(w[y], inv[y], l[x]);
-                            z[x] = fmaf(w[y], base[y], z[x]);
-                        }
-                        float back[2];
-                        a[2 * jj + x] = Elem<__half>::pack(w[0], w[1]);
-                        Elem<__half>::unpack(a[2 * jj + x], back);
-                        a2[2 * jj + x] = Elem<__half>::pack(w[0] - back[0], w[1] - back[1]);
-                    }
+                    uint32_t& hi = a[j / 2][2 * (j & 1) + x];
+                    hi = Elem<__half>::pack(w[0], w[1]);
+                    Elem<__half>::unpack(hi, back);
+                    a2[j / 2][2 * (j & 1) + x] = Elem<__half>::pack(w[0] - back[0], w[1] - back[1]);
                 }
-                const unsigned char* v = st + (BN + 8 * j + q4) * RB + g * (RB / 8);
-                uint32_t x0[NW], x1[NW];
+            }
+            // ---- O of the tile by itself, then added: an MMA truncates its sum, which the codes (none
+            // negative) would turn into a bias that grows with the keys
+            uint32_t v[NT / 2][2][NV];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const unsigned char* va = v + half * 8 * RB;
-                    const unsigned char* vb2 = va + 4 * RB;
-                    uint32_t* dst = half ? x1 : x0;
-                    if constexpr (NW % 2 == 0) {
-                        uint32_t wa[NW / 2], wb[NW / 2];
-                        if constexpr (NW % 8 == 0) {
-                            const uint4 c = *reinterpret_cast<const uint4*>(va), d = *reinterpret_cast<const uint4*>(vb2);
-                            wa[0] = c.x; wa[1] = c.y; wa[2] = c.z; wa[3] = c.w;
-                            wb[0] = d.x; wb[1] = d.y; wb[2] = d.z; wb[3] = d.w;
-                        } else if constexpr (NW % 4 == 0) {
-                            const uint2 c = *reinterpret_cast<const uint2*>(va), d = *reinterpret_cast<const uint2*>(vb2);
-                            wa[0] = c.x; wa[1] = c.y;
-                            wb[0] = d.x; wb[1] = d.y;
-                        } else {
+            for (int u = 0; u < NW; ++u) {
+                if (u % NV == 0) {
 #pragma unroll
-                            for (int i = 0; i < NW / 2; ++i) {
-                                wa[i] = *reinterpret_cast<const uint32_t*>(va + 4 * i);
-                                wb[i] = *reinterpret_cast<const uint32_t*>(vb2 + 4 * i);
-                            }
+                    for (int j = 0; j < NT / 2; ++j)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const unsigned char* at = st + (BN + 16 * j + 8 * half + q4) * RB + g * (RB / 8) + 2 * u;
+                            load_value_runs<NV>(at, at + 4 * RB, v[j][half]);
                         }
-#pragma unroll
-                        for (int i = 0; i < NW / 2; ++i) {
-                            dst[2 * i] = permute_bytes(wa[i], wb[i], 0x5410u);
-                            dst[2 * i + 1] = permute_bytes(wa[i], wb[i], 0x7632u);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < NW; ++i)
-                            dst[i] = *reinterpret_cast<const uint16_t*>(va + 2 * i) |
-                                     ((uint32_t) * reinterpret_cast<const uint16_t*>(vb2 + 2 * i) << 16);
-                    }
                 }
+                float d[4][4];
 #pragma unroll
-                for (int u = 0; u < NW; ++u) {
+                for (int j = 0; j < NT / 2; ++j) {
                     // even nibbles, and whole bytes for the odd ones (as the decode)
-                    const uint32_t l0 = x0[u] & 0x00ff00ffu, l1 = x1[u] & 0x00ff00ffu;
-                    const uint32_t h0 = permute_bytes(x0[u], 0u, 0x4341u), h1 = permute_bytes(x1[u], 0u, 0x4341u);
-                    const uint32_t m0 = l0 & kNibbleMask, m1 = l1 & kNibbleMask;
-                    const uint32_t n0 = h0 & kNibbleMask, n1 = h1 & kNibbleMask;
-                    mma16816<__half>(o[u][0], a, m0, m1);
-                    mma16816<__half>(o[u][1], a, l0, l1);
-                    mma16816<__half>(o[u][2], a, n0, n1);
-                    mma16816<__half>(o[u][3], a, h0, h1);
-                    mma16816<__half>(o[u][0], a2, m0, m1);
-                    mma16816<__half>(o[u][1], a2, l0, l1);
-                    mma16816<__half>(o[u][2], a2, n0, n1);
-                    mma16816<__half>(o[u][3], a2, h0, h1);
+                    const uint32_t v0 = v[j][0][u % NV], v1 = v[j][1][u % NV];
+                    const uint32_t l0 = v0 & 0x00ff00ffu, l1 = v1 & 0x00ff00ffu;
+                    const uint32_t h0 = permute_bytes(v0, 0u, 0x4341u), h1 = permute_bytes(v1, 0u, 0x4341u);
+                    const uint32_t b[4][2] = {{l0 & kNibbleMask, l1 & kNibbleMask}, {l0, l1},
+                                              {h0 & kNibbleMask, h1 & kNibbleMask}, {h0, h1}};
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        if (j == 0) mma16816_first(d[n], a[j], b[n][0], b[n][1]);
+                        else mma16816<__half>(d[n], a[j], b[n][0], b[n][1]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) mma16816<__half>(d[n], a2[j], b[n][0], b[n][1]);
                 }
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[u][n][i] += d[n][i];
             }
         }
         copy_wait<0>();

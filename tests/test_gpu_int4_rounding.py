@@ -280,3 +280,43 @@ def test_warps_that_share_a_unit_join_all_of_its_parts(cuda_device, heads):
     assert_rounded_once(first, expected, float(vals.max() - vals.min()) * 2.0 ** -15, torch.float16)
     for _ in range(50):
         assert torch.equal(paged_attention_int4(*args, validate=False), first)
+
+
+@pytest.mark.parametrize("form", ["decode", "twin", "prefill"])
+def test_sums_of_many_tokens_have_no_bias(cuda_device, form):
+    """The mean of (output - 64-bit value) / (the codes' part of it), over outputs of thousands of tokens each.
+
+    Sums of a tile lose at most 8 truncations of 2^-23, of which the mean is half; the tiles are added with rounding,
+    as likely up as down. The outputs' own roundings, under 2^-11 / sqrt(12) of a value that is no larger than twice
+    the codes' part, are independent: four deviations of their mean are added.
+    """
+    gen = np.random.default_rng(12)
+    bs, dim, n = 16, 64, 16384 if form == "prefill" else 32768
+    batch, kv_heads = (32, 2) if form == "prefill" else (512, 2)
+    heads = kv_heads * (2 if form == "twin" else 6)
+    rows = 64 * bs, kv_heads, dim
+    kp, vp = pool_of(keys_of_one_value(gen, *rows), bs), pool_of(rows_of_many_steps(gen, *rows), bs)
+    keys, vals = (int4_kv.values(p, bs, dim).view(-1, kv_heads, dim) for p in (kp, vp))
+    table = torch.from_numpy(gen.integers(0, 64, (batch, n // bs)).astype(np.int64))
+    query = torch.full((batch, heads, dim), 0.125, dtype=torch.float16)
+    args = query.cuda(), torch.from_numpy(kp).cuda(), torch.from_numpy(vp).cuda()
+    lens = torch.full((batch,), n)
+    if form == "prefill":
+        cu = torch.arange(batch + 1)
+        actual = paged_prefill_attention_int4(*args, cu.cuda(), (lens - 1).cuda(), table.cuda(), lens.cuda(), bs)
+    else:
+        actual = paged_attention_int4(*args, table.cuda(), lens.cuda(), bs)
+    weight = torch.exp(keys[..., 0] * math.sqrt(dim) / 8)           # [slots, kv_heads]
+    count = torch.stack([torch.bincount(t, minlength=64) for t in table]).double()
+    page = torch.einsum("pshd,psh->phd", vals.view(64, bs, kv_heads, dim), weight.view(64, bs, kv_heads))
+    low = torch.einsum("psh,psh->ph", vals.amin(-1).view(64, bs, kv_heads), weight.view(64, bs, kv_heads))
+    total = (count @ weight.view(64, bs, kv_heads).sum(1))[..., None]
+    expected = torch.einsum("bp,phd->bhd", count, page) / total
+    codes = expected - (count @ low)[..., None] / total
+    err = actual.double().cpu().view(batch, kv_heads, -1, dim) - expected[:, :, None]
+    bias = float((err / codes[:, :, None]).mean())
+    used = codes > 0.5 * expected.abs()
+    assert float(used.double().mean()) > 0.9
+    # the query heads of a kv head are alike, and so are their roundings
+    chance = 4 * 2.0 ** -11 / math.sqrt(12) * 2 / math.sqrt(batch * kv_heads * dim)
+    assert abs(bias) <= 4 * 2.0 ** -23 + chance, bias
