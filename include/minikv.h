@@ -372,8 +372,9 @@ int minikv_paged_prefill_int4(const void* q, const void* key_cache, const void* 
  * and kv head: head_dim int8 codes of the keys' elementwise maximum, head_dim of
  * their minimum, one fp32 scale = top / 127 (top: the largest magnitude of the
  * 2 * head_dim bounds), 12 zero bytes.  Codes are ceil(127 max / top) and
- * floor(127 min / top); a bound reads as code * scale.  A top below 2^-100
- * gives a zero record.  NaN keys count as 0, infinite ones as the largest fp32.
+ * floor(127 min / top); a bound reads as code * scale, and holds but for the
+ * roundings of scale and product (2^-23 of it).  A top below 2^-100 gives a zero
+ * record.  NaN keys count as 0, infinite ones as the largest fp32.
  *
  * Update the records of the blocks that hold rows [query_starts[r],
  * context_lens[r]) of each request, from all of the blocks' rows below

@@ -5,7 +5,8 @@
 // elementwise maximum over the block's rows, D of their minimum, one fp32 scale
 // (12 bytes of padding).  scale = top / 127 with top the largest magnitude of
 // the 2 D bounds; codes ceil(127 max / top) and floor(127 min / top), so that
-// code * scale bounds the keys.  A block whose top is below 2^-100 has zero
+// code * scale bounds the keys, but for the two fp32 roundings of scale and
+// product (2^-23 of the bound).  A block whose top is below 2^-100 has zero
 // codes and scale.  NaN keys count as 0, infinite ones as the largest fp32.
 //
 // Score.  For a kv head with query heads q_1 .. q_n, let qp = sum_h max(q_h, 0)
@@ -15,8 +16,10 @@
 // common to all blocks of the kv head, so
 //   score = scale_block * (sum_d maxcode_d qpcode_d + mincode_d qncode_d)
 // where the sum is a whole number below 2^24: it has one value whatever the
-// order, and with it the selection.  8-bit bounds are a sixteenth of the bytes
-// of a 16-bit block of 16 tokens (K and V: 64 D bytes).
+// order, and with it the selection.  (The codes are rounded to nearest: a score
+// stands for the bound up to half a code of each, and is not itself one.)
+// 8-bit bounds are a sixteenth of the bytes of a 16-bit block of 16 tokens (K and
+// V: 64 D bytes), and an eighth of those of a 4-bit one.
 #pragma once
 
 #include <string.h>

@@ -24,14 +24,15 @@
 // a fixed order.  A unit that spans CTAs leaves one partial per CTA; the CTA
 // that takes the unit's last ticket joins them, in the order of the CTAs.
 //
-// Long batches are bound by the instructions that make the operands: 631 a
+// Long batches are bound by the instructions that make the operands: 636 a
 // tile of 32 tokens at D = 128, where the SM could issue 760 in the time that its
 // share of the memory's rate brings the tile, and the 16 warps that the registers
-// allow keep it at half of that (256 requests of 4096 tokens, 8 kv heads: 230 us,
-// 5.0 TB/s of the pool, against 177 us at the measured copy rate).  Small ones are
-// bound by the chain of launch, look-ups, pages and join (8 x 513: 11.6 us).
+// allow keep it at half of that (256 requests of 4096 tokens, 8 kv heads: 235 us,
+// 4.9 TB/s of the pool, against 177 us at the measured copy rate; 275 in a run of
+// seconds, when the power limit takes the clock to 1650 MHz).  Small ones are
+// bound by the chain of launch, look-ups, pages and join (8 x 513: 13 us).
 // Copies a lane rather than bulk copies of a slice (1 KB of codes at D = 128):
-// those took 254 us, with more instructions, for the barriers.  mma.sync rather
+// those took a tenth longer, with more instructions, for the barriers.  mma.sync rather
 // than tcgen05: the group's few query heads are the N = 8 columns, and the
 // operands are made in registers.
 #pragma once
@@ -187,7 +188,10 @@ constexpr float kCodeScale = 16777216.f;       // 2^24: a nibble in the low bits
 // holds them twice, in columns 0..3 and again in 4..7, so the same scores and P' come
 // out there; those columns multiply the second term, and their sums are added at
 // the unit's end: no MMA more than one term takes (256 x 4096 tokens, D = 128,
-// two heads a kv head, eager: one term 269 us, this 278, a second set of MMAs 293).
+// two heads a kv head, in a long run: one term 269 us, this 278, a second set of
+// MMAs 293).  O of a tile is summed by itself and added to the unit's: 234.8 us
+// against 233.7 with MMAs that add to the unit's, at eight heads a kv head 275
+// against 258 (registers spill).
 template <typename T, int D, bool TWIN>
 struct Int4Consumer {
     static constexpr int TT = 32;
@@ -627,7 +631,8 @@ struct __align__(16) PageSlice {
     uint32_t mask;
 };
 
-// Warps of a 4-bit pool's decode work alone where each gets this many tiles, and no unit more partials than this.
+// Warps of a 4-bit pool's decode work alone where each gets this many tiles, and a unit is as long as this
+// many of their runs at most (so it has up to two partials more).
 constexpr int kLeastAlone = 5, kMostPartials = 8;
 
 // Joins n partials of a unit, in their order, into its output rows: `threads` threads share the
@@ -741,9 +746,9 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 
     // turn and join at the end of each unit, or a single warp with a run of its own: no barrier, an
     // eighth of the joins, but a unit is then cut into as many partials as warps share it.  The figures
     // come from the lengths, so all CTAs agree.  A CTA and a warp, D = 128, 8 kv heads: 256 x 4096 tokens
-    // (111 tiles a warp, 2 partials) 266 and 230 us, 64 x 4096 (28, 5) 82 and 75, 64 lists of 1024 (7, 5)
-    // 37 and 33, 32 x 4096 (14, 10) 49 and 47, 32 lists of 2048 (7, 10) 33 and 35, 12 x 4096 (5, 25) 29 and
-    // 31, 32 x 1024 (3.5, 10) 19 and 23, 1 x 131072 (14, 296) 47 and 108.  A 16-bit pool's four warps are
+    // (111 tiles a warp, a unit of 1.2 runs) 274 and 235 us, 64 x 4096 (28, 5) 82 and 73, 64 lists of 1024
+    // (7, 5) 37 and 31, 32 x 4096 (14, 9) 48 and 46, 32 lists of 2048 (7, 9) 33 and 31, 12 x 4096 (5, 25) 27
+    // and 29, 32 x 1024 (3.5, 9) 17 and 22, 1 x 131072 (14, 296) 46 and 102.  A 16-bit pool's four warps are
     // faster together: 64 lists of 2048 tokens 99 and 101 us, 32 of them 57 and 61.
     const int64_t total = (int64_t)prefix[W * 32] * U;
     int longest = 0;
@@ -755,7 +760,7 @@ __global__ void __launch_bounds__(PageShape<Consumer, INT4>::kThreads, D <= 128 
     const int64_t team = alone ? (int64_t)blockIdx.x * W + warp : blockIdx.x;
     int64_t G = (int64_t)gridDim.x * (alone ? W : 1);  // runs
     // Every run has a tile, of a CTA at least one for each warp; where that is no more than four a warp,
-    // a whole unit's, which then needs no join (8 x 513 tokens: 17.8 -> 11.6 us).
+    // a whole unit's, which then needs no join (8 x 513 tokens: 17.8 -> 11.6 us when it was introduced).
     const int least = longest <= 4 * W ? max(W, longest) : W;
     G = min(G, alone ? total : (total + least - 1) / least);
     if (team >= G) return;

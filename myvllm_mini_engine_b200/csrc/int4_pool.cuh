@@ -121,8 +121,8 @@ __device__ __forceinline__ uint32_t int4_code(float x, float base, float step) {
 // Quantising write.  A unit is one row: (token, kv head, K or V); a group of
 // int4_row_lanes(D, 16) lanes takes one, 16 elements a lane, so at D = 128 a
 // warp takes the K and the V rows of two heads of a token (8 elements a lane,
-// twice the row's own work an element, took 46 us for 16384 tokens of 8 heads in
-// fp16 where this takes 34: 2.5 TB/s, bound by issue).  The usual row costs an
+// twice the row's own work an element, took a third longer).  Bound by issue: 75 %
+// of the slots used; 16384 tokens of 8 heads of 128 in fp16 28.7 us, 3.0 TB/s.  The usual row costs an
 // element a subtraction, two products with the rounded inverse of the step (a
 // little above and a little below it, each rounded to a whole number by an
 // addition of 1.5 2^23) and an addition into the word: where the two agree, so

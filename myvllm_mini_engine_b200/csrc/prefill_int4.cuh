@@ -14,9 +14,12 @@
 // P' enters in two fp16 terms (2^-22): one (2^-12) would move half of an fp16
 // output's roundings to the next value, and a twentieth of a bf16 one's (4 x 1000
 // tokens behind 4096, 32/8 heads of 128: 1181 us with one term, 1515 with two).
+// O of a tile of keys is summed by itself and then added (the same: 1473 us with
+// MMAs that add to the row's, 1593 so).
 //
-// Bound by the tensor pipe and by issue: a warp makes its operands from the
-// codes itself.  mma.sync rather than tcgen05: a tcgen05 operand has to lie in
+// Bound by the tensor pipe (48 % of its cycles), by issue (40 %) and by the
+// latencies that 8 warps a SM leave open: a warp makes its operands from the codes
+// itself.  mma.sync rather than tcgen05: a tcgen05 operand has to lie in
 // shared memory as 16-bit values, four times the codes' bytes written there and
 // read back per tile, while the masked registers feed mma.sync as they are and
 // the P operand never leaves them.
@@ -69,9 +72,9 @@ __device__ __forceinline__ void load_value_runs(const unsigned char* a, const un
     }
 }
 
-// CTAs a SM: three at 64 dims or fewer (4 x 1000 tokens behind 4096, 32/8 heads of 64: 878 us, with two
-// 927); at 96 and 128 the registers of three spill, and two take 1473 against 1500 us at 128, and 32 x 8
-// tokens behind 2048 with 16/8 heads 100 against 152.
+// CTAs a SM: three at 64 dims or fewer (4 x 1000 tokens behind 4096, 32/8 heads of 64: 916 us, with two
+// 992; though 32 x 8 behind 2048, 16/8 heads, 92 and 69); at 96 and 128 the registers of three spill, and two
+// take 1592 against 1645 us at 128, and 32 x 8 tokens 108 against 166.
 template <typename T, int D>
 __global__ void __launch_bounds__(kPrefillThreads, D <= 64 ? 3 : 2) prefill_int4_kernel(const PrefillInt4Params p) {
     constexpr int BN = D <= 128 ? 64 : 32;  // keys a tile: the accumulators of S take BN / 2 registers

@@ -12,10 +12,11 @@ request get next to no weight.  Three steps read only those that can matter:
 
 Bounds are a contiguous uint8 tensor ``[num_blocks, kv_heads, 2 * head_dim + 16]``:
 ``head_dim`` int8 codes of the keys' elementwise maximum, ``head_dim`` of their
-minimum, one fp32 scale; a bound reads as ``code * scale``.  A score is a bound of
-``sum_h q_h . k`` over the query heads h of a kv head and the keys k of the block;
-the codes' products sum to a whole number, so a selection is the same whatever
-the batch, the split or the order of evaluation.
+minimum, one fp32 scale; a bound reads as ``code * scale`` (it holds up to two fp32
+roundings, 2^-23 of it).  A score estimates the bound of ``sum_h q_h . k`` over the
+query heads h of a kv head and the keys k of the block, with the query's parts
+rounded to 8 bits; the codes' products sum to a whole number, so a selection is
+the same whatever the batch, the split or the order of evaluation.
 """
 
 from __future__ import annotations
