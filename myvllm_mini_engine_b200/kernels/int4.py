@@ -23,6 +23,8 @@ has its own.
 
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from .. import _lib
@@ -234,6 +236,7 @@ _SCRATCH: dict = {}
 _OLD_SCRATCH: list = []
 _CAPTURED: dict = {}
 _CAPTURED_TICKETS = 1 << 22
+_CAPTURED_LOCK = threading.Lock()
 
 
 def _captured_tickets(device, count):
@@ -244,9 +247,12 @@ def _captured_tickets(device, count):
     holds counters that it zeroes itself, about 2 us a call.
     """
     held = _CAPTURED.get(device.index)
-    if held is None or held[1] + count > held[0].numel():
+    with _CAPTURED_LOCK:
+        first = -1
+        if held is not None and held[1] + count <= held[0].numel():
+            first, held[1] = held[1], held[1] + count
+    if first < 0:
         return torch.zeros(count, dtype=torch.int32, device=device)
-    first, held[1] = held[1], held[1] + count
     return held[0][first:first + count]
 
 

@@ -43,3 +43,35 @@ def test_pools_tell_the_bytes_of_their_bounds():
         assert plain.bounds_bytes == 0 and held.memory_bytes == plain.memory_bytes
         assert held.bounds_bytes == 2 * 5 * 3 * (2 * 128 + 16) == held.bounds.nbytes
         assert held.memory_bytes // held.bounds_bytes == share
+
+
+def test_captures_of_two_threads_where_the_kept_counters_end(monkeypatch):
+    """A second capture that comes in between the first one's look at what is left and its taking it."""
+    import threading
+
+    from myvllm_mini_engine_b200.kernels import int4
+
+    device, count, got = torch.device("cpu", 0), 3, []
+
+    class Kept:
+        """Counters for one call more."""
+
+        def __init__(self):
+            self.data, self.other = torch.zeros(count, dtype=torch.int32), None
+
+        def numel(self):
+            if self.other is None:
+                self.other = threading.Thread(target=lambda: got.append(int4._captured_tickets(device, count)))
+                self.other.start()
+                self.other.join(0.3)
+            return self.data.numel()
+
+        def __getitem__(self, part):
+            return self.data[part]
+
+    kept = Kept()
+    monkeypatch.setattr(int4, "_CAPTURED", {0: [kept, 0]})
+    got.append(int4._captured_tickets(device, count))
+    kept.other.join(5)
+    assert len(got) == 2 and all(t.numel() == count for t in got)
+    assert got[0].data_ptr() != got[1].data_ptr()
